@@ -1,0 +1,620 @@
+"""The operators around a paged key-value cache, as a serving program calls them.
+
+  rotary   apply_rotary turns queries and keys by their positions; append_paged
+           does it while it writes the new keys and values into their pages
+  paged    attend_paged: one new token per sequence over its pages, scores
+           capped by a tanh or biased by distance, in a window, behind a prefix
+  prompt   attend_prompt: causal attention of whole prompts with the same
+           changes to the scores, several documents packed in a row
+  fork     fork_pages: sequences become children of others (beams, shared
+           prompts, ended ones), with pages for their next tokens
+  evict    evict_pages: the pages of evicted 64-token tiles leave the tables
+
+listed() holds the cases, draw() gives more of the same ranges, prepare()
+makes a case's inputs on the GPU, run() is one pass, work() the bytes and
+operations a pass cannot do without, exact() the outputs in 64 bits.  Lengths
+and documents are drawn from the case's own sizes, values from the seed.
+"""
+
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+DEV = "cuda"
+TILE = 64
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "fp8": torch.float8_e4m3fn}
+BYTES = {"f32": 4, "f16": 2, "bf16": 2, "fp8": 1}
+
+
+def listed():
+    return [
+        # one layer's queries and keys after the projections of a 4096-token prompt, (batch, tokens, heads, dim) in memory
+        {"name": "rotary_4k_bf16", "kind": "rotary", "batch": 1, "heads": 32, "rows": 8, "tokens": 4096, "dim": 128,
+         "turned": 128, "layout": "half", "first": 0, "dtype": "bf16", "backward": False},
+        # a decode step of 16 sequences: one token each is turned and stored; all latency
+        {"name": "append_step_bf16", "kind": "append", "seqs": 16, "fresh": 1, "cached": 4096, "heads": 32, "rows": 8,
+         "dim": 128, "turned": 128, "layout": "half", "first": 0, "page": 16, "dtype": "bf16", "cache": "bf16"},
+        # ragged prompt chunks far into long contexts, half of each head turned in pairs, stored in 8 bits
+        {"name": "append_chunks_fp8", "kind": "append", "seqs": 9, "fresh": 1500, "cached": 5000, "heads": 32, "rows": 8,
+         "dim": 128, "turned": 64, "layout": "interleaved", "first": 120000, "page": 32, "dtype": "bf16", "cache": "fp8"},
+        # three short sequences, the smallest decode: 32 query heads on 4, scores capped
+        {"name": "paged_short_f16", "kind": "paged", "seqs": 3, "tokens": 300, "heads": 32, "rows": 4, "dim": 64,
+         "page": 16, "dtype": "f16", "cache": "f16", "cap": 30.0, "bias": False, "window": 0, "prefix": 0, "evict": 0.0},
+        # serving: 16 sequences of up to 32K tokens, scores falling with distance
+        {"name": "paged_16_bf16", "kind": "paged", "seqs": 16, "tokens": 32768, "heads": 32, "rows": 8, "dim": 128,
+         "page": 16, "dtype": "bf16", "cache": "bf16", "cap": 0.0, "bias": True, "window": 0, "prefix": 0, "evict": 0.0},
+        # long contexts in 8 bits, 64 query heads on 8, scores capped
+        {"name": "paged_128k_fp8", "kind": "paged", "seqs": 4, "tokens": 131072, "heads": 64, "rows": 8, "dim": 128,
+         "page": 64, "dtype": "bf16", "cache": "fp8", "cap": 50.0, "bias": False, "window": 0, "prefix": 0, "evict": 0.0},
+        # the prompt of one layer, scores capped
+        {"name": "prompt_4k_bf16", "kind": "prompt", "batch": 1, "heads": 32, "rows": 8, "tokens": 4096, "dim": 128,
+         "dtype": "bf16", "cap": 50.0, "bias": False, "window": 0, "prefix": 0, "docs": 1},
+        # documents of all lengths packed into a row of odd length, scores falling with distance
+        {"name": "prompt_docs_8k_f16", "kind": "prompt", "batch": 1, "heads": 32, "rows": 8, "tokens": 8191, "dim": 128,
+         "dtype": "f16", "cap": 0.0, "bias": True, "window": 0, "prefix": 0, "docs": 9},
+        # eight beams of one layer are reordered
+        {"name": "fork_beams_bf16", "kind": "fork", "seqs": 8, "tokens": 700, "layers": 1, "rows": 8, "dim": 128,
+         "page": 16, "cache": "bf16", "fresh": 1},
+        # 64 sequences over the pages of 16 layers: some end, others get several children, each with its last page
+        {"name": "fork_64_layers_bf16", "kind": "fork", "seqs": 64, "tokens": 600, "layers": 16, "rows": 8, "dim": 128,
+         "page": 64, "cache": "bf16", "fresh": 100},
+        # the tiles that every head of eight short sequences evicts leave the tables
+        {"name": "evict_8", "kind": "evict", "seqs": 8, "tokens": 4096, "rows": 8, "page": 16, "evict": 0.5},
+        # the same for 256 sequences of up to 32K tokens
+        {"name": "evict_256", "kind": "evict", "seqs": 256, "tokens": 32768, "rows": 8, "page": 16, "evict": 0.5},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(("rotary", "append", "paged", "paged", "prompt", "prompt", "fork", "evict"))
+    rows = rng.choice((1, 2, 4, 8))
+    group = rng.choice((1, 3, 4, 8))
+    dim = rng.choice((64, 128))
+    page = rng.choice((16, 32, 64))
+    if kind in ("rotary", "append"):
+        c = {"kind": kind, "heads": rows * group, "rows": rows, "dim": dim, "turned": rng.choice((dim, dim // 2)),
+             "layout": rng.choice(("half", "interleaved")), "first": rng.choice((0, 1, 777, 200000)),
+             "dtype": rng.choice(("f32", "f16", "bf16"))}
+        if kind == "rotary":
+            return {**c, "batch": rng.choice((1, 2, 3)), "tokens": _log_int(rng, 1, 4096), "backward": rng.random() < 0.5}
+        c["cache"] = rng.choice((c["dtype"], "fp8"))
+        return {**c, "seqs": _log_int(rng, 1, 32), "fresh": _log_int(rng, 1, 1024), "cached": _log_int(rng, 1, 4096),
+                "page": page}
+    change = {"cap": rng.choice((0.0, 20.0, 50.0)), "bias": rng.random() < 0.4,
+              "window": rng.choice((0, 0, 129, 1024)), "prefix": rng.choice((0, 0, 40, 200))}
+    if kind == "paged":
+        dtype, seqs, dim = rng.choice(("f32", "f16", "bf16", "bf16")), _log_int(rng, 1, 32), rng.choice((64, 128, 128, 256))
+        cache = rng.choice((dtype, "fp8"))
+        most = min(131072, 500000000 // (seqs * rows * dim * BYTES[cache]))
+        return {"kind": kind, "seqs": seqs, "tokens": _log_int(rng, 20, most), "heads": rows * group, "rows": rows,
+                "dim": dim, "page": page, "dtype": dtype, "cache": cache, **change, "evict": rng.choice((0.0, 0.0, 0.5))}
+    if kind == "prompt":
+        batch = rng.choice((1, 2))
+        tokens = _log_int(rng, 17, min(8192, int(4096 * math.sqrt(32 / (batch * rows * group)))))
+        return {"kind": kind, "batch": batch, "heads": rows * group, "rows": rows, "tokens": tokens,
+                "dim": dim, "dtype": rng.choice(("f32", "f16", "bf16")), **change,
+                "docs": rng.choice((1, 1, min(4, tokens // 8), min(7, tokens // 2)))}
+    if kind == "fork":
+        return {"kind": kind, "seqs": _log_int(rng, 2, 64), "tokens": _log_int(rng, 40, 4096), "layers": rng.choice((1, 2, 5)),
+                "rows": rows, "dim": dim, "page": page, "cache": rng.choice(("f32", "bf16", "fp8")),
+                "fresh": rng.choice((0, 1, 100))}
+    return {"kind": kind, "seqs": _log_int(rng, 1, 128), "tokens": _log_int(rng, 100, 32768), "rows": rows, "page": page,
+            "evict": rng.choice((0.2, 0.5, 0.8))}
+
+
+# ---------------------------------------------------------------- sizes that a case fixes
+
+def _sizes(case):
+    """A generator of the case's lengths: the same for every seed."""
+    return random.Random(repr(sorted((k, v) for k, v in case.items() if k != "name")))
+
+
+def _lens(case, key="tokens", low=0.3):
+    """Tokens per sequence: from a share of the case's most up to it, one of them the most."""
+    r, most = _sizes(case), case[key]
+    lens = [max(1, int(most * r.uniform(low, 1.0))) for _ in range(case["seqs"])]
+    lens[r.randrange(len(lens))] = most
+    return lens
+
+
+def _fresh(case):
+    """New tokens per sequence of an append: all alike in a step, else ragged (one sequence may have none)."""
+    if case["fresh"] == 1:
+        return [1] * case["seqs"]
+    r = random.Random(case["fresh"] * 7 + case["seqs"])
+    return [max(0, int(case["fresh"] * r.uniform(-0.05, 1.0))) for _ in range(case["seqs"] - 1)] + [case["fresh"]]
+
+
+def _doc_ids(case):
+    """Document of every token of a packed row."""
+    r, n, docs = random.Random(case["tokens"] * 31 + case["docs"]), case["tokens"], case["docs"]
+    cuts = sorted(r.sample(range(1, n), docs - 1)) if docs > 1 else []
+    return [i for i, (a, b) in enumerate(zip([0] + cuts, cuts + [n])) for _ in range(b - a)]
+
+
+def _parents(case):
+    """The parent of every child: some sequences end, others have several children."""
+    r, n = _sizes(case), case["seqs"]
+    kept = r.sample(range(n), max(1, (2 * n) // 3))
+    return [r.choice(kept) if r.random() < 0.95 else -1 for _ in range(n)]
+
+
+# ---------------------------------------------------------------- inputs
+
+def _normal(g, shape, dtype):
+    return torch.randn(shape, generator=g, device=DEV, dtype=torch.float32).to(DTYPES[dtype])
+
+
+def _frequencies(turned):
+    """Turns per position of each pair, a base of 500000 as in models for long contexts."""
+    i = torch.arange(turned // 2, dtype=torch.float64, device=DEV)
+    return torch.pow(torch.tensor(500000.0, dtype=torch.float64, device=DEV), -2.0 * i / turned)
+
+
+def _tables(g, pages, num_blocks):
+    """(seqs, most) tables of distinct pages in random order, -1 past a sequence's own."""
+    count = torch.tensor(pages, device=DEV)
+    most = max(pages)
+    at = torch.arange(most, device=DEV)[None, :]
+    slot = count.cumsum(0)[:, None] - count[:, None] + at
+    order = torch.randperm(num_blocks, generator=g, device=DEV)
+    return torch.where(at < count[:, None], order[slot.clamp(max=num_blocks - 1)], -1).to(torch.int32).contiguous()
+
+
+def _int(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    c = dict(case)
+    kind, s = c["kind"], {"case": c}
+    if kind == "rotary":
+        for name, heads in (("q", c["heads"]), ("k", c["rows"])):
+            s[name] = _normal(g, (c["batch"], c["tokens"], heads, c["dim"]), c["dtype"]).transpose(1, 2)
+        s["positions"] = c["first"] + torch.arange(c["tokens"], device=DEV, dtype=torch.int32)
+        s["freq"] = _frequencies(c["turned"])
+        return s
+    if kind == "append":
+        fresh, cached, page = _fresh(c), _lens(c, "cached"), c["page"]
+        pages = [-(-(a + b) // page) for a, b in zip(cached, fresh)]
+        total, num_blocks = sum(fresh), sum(pages) + 8
+        for name, heads in (("q", c["heads"]), ("k", c["rows"]), ("v", c["rows"])):
+            s[name] = _normal(g, (total, heads, c["dim"]), c["dtype"])
+        for name in ("k_cache", "v_cache"):
+            s[name] = _normal(g, (num_blocks, c["rows"], page, c["dim"]), c["cache"])
+        s["tables"], s["lens"] = _tables(g, pages, num_blocks), _int(cached)
+        s["cu"] = None if c["fresh"] == 1 else _int([sum(fresh[:i]) for i in range(len(fresh) + 1)])
+        # positions of the tokens: they run ahead of the slots where tiles were evicted before
+        s["positions"] = _int([c["first"] + a + i for a, b in zip(cached, fresh) for i in range(b)])
+        s["freq"] = _frequencies(c["turned"])
+        s["k_scale"], s["v_scale"] = (0.02, 0.015) if c["cache"] == "fp8" else (1.0, 1.0)
+        return s
+    if kind == "paged":
+        lens, page = _lens(c), c["page"]
+        pages = [-(-n // page) for n in lens]
+        num_blocks = sum(pages) + 8
+        s["q"] = _normal(g, (c["seqs"], c["heads"], c["dim"]), c["dtype"])
+        for name in ("k_cache", "v_cache"):
+            s[name] = torch.empty((num_blocks, c["rows"], page, c["dim"]), device=DEV, dtype=DTYPES[c["cache"]])
+            for b in range(0, num_blocks, 4096):  # in parts, to stay small in 32 bits
+                part = s[name][b:b + 4096]
+                part.copy_(_normal(g, part.shape, "f32"))
+        s["tables"], s["lens"] = _tables(g, pages, num_blocks), _int(lens)
+        s["k_scale"], s["v_scale"] = (1.3, 0.8) if c["cache"] == "fp8" else (1.0, 1.0)
+        s["slopes"] = _slopes(c["heads"]) if c["bias"] else None
+        s["prefix"] = _int([(c["prefix"] * (i + 1)) // c["seqs"] for i in range(c["seqs"])]) if c["prefix"] else None
+        s["evict"] = None
+        if c["evict"]:
+            s["evict"] = torch.rand((c["seqs"], c["rows"], max(1, -(-max(lens) // TILE))), generator=g, device=DEV) < c["evict"]
+        return s
+    if kind == "prompt":
+        for name, heads in (("q", c["heads"]), ("k", c["rows"]), ("v", c["rows"])):
+            s[name] = _normal(g, (c["batch"], c["tokens"], heads, c["dim"]), c["dtype"]).transpose(1, 2)
+        s["slopes"] = _slopes(c["heads"]) if c["bias"] else None
+        s["prefix"] = _int([min(c["prefix"] + i, c["tokens"]) for i in range(c["batch"])]) if c["prefix"] else None
+        s["docs"] = _int([_doc_ids(c)] * c["batch"]) if c["docs"] > 1 else None
+        return s
+    lens, page = _lens(c), c["page"]
+    if kind == "fork":
+        pages, parents = [-(-n // page) for n in lens], _parents(c)
+        fresh = [c["fresh"]] * c["seqs"]
+        spare = sum(1 + -(-n // page) for n in fresh)
+        num_blocks = sum(pages) + spare
+        for name in ("k_cache", "v_cache"):
+            s[name] = torch.empty((c["layers"], num_blocks, c["rows"], page, c["dim"]), device=DEV, dtype=DTYPES[c["cache"]])
+            for layer in range(c["layers"]):
+                s[name][layer].copy_(_normal(g, s[name].shape[1:], "f32"))
+        room = max(-(-(n + c["fresh"]) // page) for n in lens)
+        tables = torch.nn.functional.pad(_tables(g, pages, num_blocks), (0, room - max(pages)), value=-1)
+        s["parents"], s["fresh"] = _int(parents), _int(fresh)
+    else:
+        pages = [-(-n // page) for n in lens]
+        num_blocks = sum(pages) + 8
+        tables = _tables(g, pages, num_blocks)
+        tiles = -(-max(lens) // TILE)
+        # heads agree on most tiles: a tile leaves when all of them evict it
+        base = torch.rand((c["seqs"], 1, tiles), generator=g, device=DEV) < c["evict"]
+        other = torch.rand((c["seqs"], c["rows"], tiles), generator=g, device=DEV) < 0.02
+        s["evict"] = base ^ other
+    s["tables"], s["lens"] = tables.contiguous(), _int(lens)
+    s["refs"] = torch.zeros(num_blocks, dtype=torch.int32, device=DEV)
+    s["refs"].index_put_((tables[tables >= 0].long(),), torch.ones((), dtype=torch.int32, device=DEV), accumulate=True)
+    return s
+
+
+def _slopes(heads):
+    """Slopes of the distance bias: a geometric row over the heads."""
+    return torch.pow(2.0, -8.0 * (torch.arange(heads, device=DEV, dtype=torch.float32) + 1) / heads)
+
+
+# ---------------------------------------------------------------- the plain forms
+
+def _turn(x, positions, freq, turned, layout, backward):
+    """x (..., tokens, dim) in float32, turned by its positions."""
+    angle = positions.double()[..., None] * freq
+    cos, sin = angle.cos().float(), angle.sin().float()
+    if backward:
+        sin = -sin
+    t, rest = x[..., :turned], x[..., turned:]
+    if layout == "half":
+        a, b = t[..., :turned // 2], t[..., turned // 2:]
+        t = torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+    else:
+        a, b = t[..., 0::2], t[..., 1::2]
+        t = torch.stack((a * cos - b * sin, b * cos + a * sin), -1).flatten(-2)
+    return torch.cat((t, rest), -1)
+
+
+def _stored(x, scale, cache):
+    """x as the cache holds it, as raw values."""
+    if cache.dtype == torch.float8_e4m3fn:
+        return (x / scale).clamp(-448.0, 448.0).to(cache.dtype).view(torch.uint8), cache.view(torch.uint8)
+    return x.to(cache.dtype), cache
+
+
+def _plain_append(s):
+    c, n = s["case"], s["k"].shape[0]
+    row = torch.arange(n, device=DEV)
+    if s["cu"] is None:
+        seq, at = row, s["lens"].long()
+    else:
+        seq = torch.searchsorted(s["cu"].long(), row, right=True) - 1
+        at = s["lens"].long()[seq] + row - s["cu"].long()[seq]
+    page = s["tables"][seq, at // c["page"]].long()
+    slot = at % c["page"]
+    q, k = (_turn(s[i].float().transpose(0, 1), s["positions"], s["freq"], c["turned"], c["layout"], False).transpose(0, 1)
+            for i in ("q", "k"))
+    kv, kc = _stored(k, s["k_scale"], s["k_cache"])
+    vv, vc = _stored(s["v"].float(), s["v_scale"], s["v_cache"])
+    kc[page, :, slot] = kv
+    vc[page, :, slot] = vv
+    return {"q": q.to(s["q"].dtype), "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
+
+
+def _softmax(scores, seen):
+    """Softmax over the seen places of the last dimension; all zeros where none is."""
+    scores = scores.masked_fill(~seen, -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    p = torch.exp(scores - top.masked_fill(top == -math.inf, 0.0))
+    return p / p.sum(-1, keepdim=True).clamp(min=1e-30)
+
+
+def _changed(scores, c, slopes, distance):
+    """The scores capped, then biased by distance."""
+    if c["cap"]:
+        scores = c["cap"] * torch.tanh(scores / c["cap"])
+    return scores if slopes is None else scores - slopes * distance
+
+
+def _plain_paged(s):
+    c, lens = s["case"], s["lens"].long()
+    n, rows, group = c["seqs"], c["rows"], c["heads"] // c["rows"]
+
+    def rows_of(cache, scale):
+        x = cache.view(torch.uint8) if cache.element_size() == 1 else cache
+        x = x[s["tables"].long().clamp(min=0)].view(cache.dtype).float() * scale
+        return x.transpose(1, 2).reshape(n, rows, -1, c["dim"])
+
+    k, v = rows_of(s["k_cache"], s["k_scale"]), rows_of(s["v_cache"], s["v_scale"])
+    j = torch.arange(k.shape[2], device=DEV)
+    distance = (lens[:, None] - 1 - j).view(n, 1, 1, -1)
+    seen = distance >= 0
+    if c["window"]:
+        near = distance < c["window"]
+        if s["prefix"] is not None:
+            near = near | (j < s["prefix"][:, None]).view(n, 1, 1, -1)
+        seen = seen & near
+    if s["evict"] is not None:
+        tile = (j // TILE).clamp(max=s["evict"].shape[2] - 1)
+        whole = ((j // TILE + 1) * TILE <= lens[:, None]).view(n, 1, 1, -1)
+        seen = seen & ~(s["evict"][:, :, tile].view(n, rows, 1, -1) & whole)
+    scores = torch.matmul(s["q"].float().view(n, rows, group, c["dim"]), k.transpose(2, 3)) / math.sqrt(c["dim"])
+    slopes = None if s["slopes"] is None else s["slopes"].view(1, rows, group, 1)
+    p = _softmax(_changed(scores, c, slopes, distance), seen)
+    return torch.matmul(p, v).view(n, c["heads"], c["dim"]).to(s["q"].dtype)
+
+
+def _plain_prompt(s):
+    c, t = s["case"], s["case"]["tokens"]
+    group = c["heads"] // c["rows"]
+    q, k, v = (s[i].float() for i in ("q", "k", "v"))
+    at = torch.arange(t, device=DEV)
+    distance = at[:, None] - at[None, :]
+    seen = distance >= 0
+    if c["window"]:
+        seen = seen & (distance < c["window"])
+    seen = seen.view(1, 1, 1, t, t)
+    if s["prefix"] is not None:
+        seen = seen | (at < s["prefix"][:, None]).view(-1, 1, 1, 1, t)
+    if s["docs"] is not None:
+        seen = seen & (s["docs"][:, :, None] == s["docs"][:, None, :]).view(-1, 1, 1, t, t)
+    scores = torch.matmul(q.unflatten(1, (c["rows"], group)), k.unsqueeze(2).transpose(-1, -2)) / math.sqrt(c["dim"])
+    slopes = None if s["slopes"] is None else s["slopes"].view(1, c["rows"], group, 1, 1)
+    p = _softmax(_changed(scores, c, slopes, distance.abs()), seen)
+    return torch.matmul(p, v.unsqueeze(2)).flatten(1, 2).to(s["q"].dtype)
+
+
+def _plain_fork(s):
+    c, page = s["case"], s["case"]["page"]
+    tables, lens, refs, parents = s["tables"], s["lens"].long(), s["refs"], s["parents"].long()
+    n, most = tables.shape
+    real = parents >= 0
+    parent = parents.clamp(min=0)
+    child = (parents[:, None] == torch.arange(n, device=DEV)) & real[:, None]  # (children, parents)
+    count = child.sum(0)
+    at = torch.arange(parents.shape[0], device=DEV)
+    first = torch.where(child, at[:, None], parents.shape[0]).amin(0)  # the first child of each parent
+    new_len = torch.where(real, lens[parent], 0)
+    full, part = new_len // page, new_len % page
+    last = tables[parent].gather(1, full.clamp(max=most - 1)[:, None])[:, 0].long()
+    alone = refs[last.clamp(min=0)] <= 1
+    copied = (part > 0) & ~((first[parent] == at) & alone)
+    have = full + (part > 0) - copied.long()       # pages that the child takes from its parent
+    need = torch.where(real, -(-(new_len + s["fresh"]) // page), 0)
+    take = need - have
+    free = torch.nonzero(refs == 0)[:, 0]
+    start = take.cumsum(0) - take
+    col = torch.arange(most, device=DEV)
+    fresh = free[(start[:, None] + col - have[:, None]).clamp(0, free.shape[0] - 1)]
+    new = torch.where(col < have[:, None], tables[parent].long(), torch.where(col < need[:, None], fresh, -1))
+    # counts: one less for what a parent held, one more for what a child holds
+    change = torch.zeros(refs.shape[0] + 1, dtype=torch.int64, device=DEV)
+    held, got = tables.long(), new
+    change.index_put_((torch.where(held >= 0, held, refs.shape[0]).flatten(),), torch.tensor(-1, device=DEV), accumulate=True)
+    change.index_put_((torch.where(got >= 0, got, refs.shape[0]).flatten(),), torch.tensor(1, device=DEV), accumulate=True)
+    # the tokens of copied pages (the others copy a slot of their own onto itself)
+    to = new.gather(1, full.clamp(max=most - 1)[:, None])[:, 0]
+    src = torch.where(copied, last, to.clamp(min=0)).clamp(min=0)
+    dst = torch.where(copied, to, src)
+    pick = torch.nonzero(copied)[:, 0]
+    used = (torch.arange(page, device=DEV) < part[pick][:, None]).view(1, -1, 1, page, 1)
+    for cache in (s["k_cache"], s["v_cache"]):
+        raw = cache.view(torch.uint8) if cache.element_size() == 1 else cache
+        raw[:, dst[pick]] = torch.where(used, raw[:, src[pick]], raw[:, dst[pick]])
+    return {"tables": new.to(torch.int32), "lens": new_len.to(torch.int32), "refs": (refs + change[:-1]).to(torch.int32),
+            "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
+
+
+def _plain_evict(s):
+    page, per = s["case"]["page"], TILE // s["case"]["page"]
+    tables, lens, refs = s["tables"].long(), s["lens"].long(), s["refs"]
+    n, most = tables.shape
+    tiles = -(-most * page // TILE)
+    t = torch.arange(tiles, device=DEV)
+    gone = s["evict"].all(1)
+    gone = torch.nn.functional.pad(gone, (0, max(0, tiles - gone.shape[1])))[:, :tiles] & ((t + 1) * TILE <= lens[:, None])
+    kept = ~gone & (t * TILE < lens[:, None])
+    order = torch.sort(torch.where(kept, t, tiles + t), 1).values  # kept tiles in order, then the others
+    tile_map = torch.where(order < tiles, order, -1)
+    new_len = lens - gone.sum(1) * TILE
+    col = torch.arange(most, device=DEV)
+    src = tile_map[:, col // per] * per + col % per
+    used = col < (-(-new_len // page))[:, None]
+    new = torch.where(used, tables.gather(1, src.clamp(0, most - 1)), -1)
+    change = torch.zeros(refs.shape[0] + 1, dtype=torch.int64, device=DEV)
+    change.index_put_((torch.where(tables >= 0, tables, refs.shape[0]).flatten(),), torch.tensor(-1, device=DEV), accumulate=True)
+    change.index_put_((torch.where(new >= 0, new, refs.shape[0]).flatten(),), torch.tensor(1, device=DEV), accumulate=True)
+    return {"tables": new.to(torch.int32), "lens": new_len.to(torch.int32), "refs": (refs + change[:-1]).to(torch.int32),
+            "tile_map": tile_map.to(torch.int32)}
+
+
+def _plain(s):
+    kind, c = s["case"]["kind"], s["case"]
+    if kind == "rotary":
+        return [_turn(s[i].float(), s["positions"], s["freq"], c["turned"], c["layout"], c["backward"]).to(s[i].dtype)
+                for i in ("q", "k")]
+    return {"append": _plain_append, "paged": _plain_paged, "prompt": _plain_prompt, "fork": _plain_fork,
+            "evict": _plain_evict}[kind](s)
+
+
+# ---------------------------------------------------------------- the framework's operators
+
+def _framework():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "orthocache-gpu_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import orthocache_gpu
+    return orthocache_gpu
+
+
+def _own(s):
+    oc, c = _framework(), s["case"]
+    kind = c["kind"]
+    if kind in ("rotary", "append"):
+        table = oc.RotaryTable(s["freq"])
+        if kind == "rotary":
+            return list(oc.apply_rotary(s["q"], s["k"], s["positions"], table, layout=c["layout"], backward=c["backward"]))
+        q = oc.append_paged(s["k"], s["v"], s["k_cache"], s["v_cache"], s["tables"], s["lens"], q=s["q"],
+                            cu_seqlens=s["cu"], positions=s["positions"], table=table, layout=c["layout"],
+                            k_scale=s["k_scale"], v_scale=s["v_scale"], sync=False)
+        return {"q": q, "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
+    if kind == "paged":
+        return oc.attend_paged(s["q"], s["k_cache"], s["v_cache"], s["tables"], s["lens"], softcap=c["cap"],
+                               alibi_slopes=s["slopes"], window=c["window"], prefix_lens=s["prefix"],
+                               k_scale=s["k_scale"], v_scale=s["v_scale"], evict_mask=s["evict"], sync=False)
+    if kind == "prompt":
+        return oc.attend_prompt(s["q"], s["k"], s["v"], softcap=c["cap"], alibi_slopes=s["slopes"], window=c["window"],
+                                prefix_lens=s["prefix"], documents=s["docs"])
+    if kind == "fork":
+        r = oc.fork_pages(s["k_cache"], s["v_cache"], s["tables"], s["lens"], s["refs"], parents=s["parents"],
+                          new_tokens=s["fresh"], sync=False)
+        return {"tables": r.block_tables, "lens": r.context_lens, "refs": r.ref_counts, "k_cache": s["k_cache"],
+                "v_cache": s["v_cache"]}
+    r, tile_map = oc.evict_pages(s["tables"], s["lens"], s["refs"], s["evict"], block_size=c["page"], sync=False)
+    return {"tables": r.block_tables, "lens": r.context_lens, "refs": r.ref_counts, "tile_map": tile_map}
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+# ---------------------------------------------------------------- what a pass cannot do without
+
+def _seen_pairs(case):
+    """Scores of a prompt's rows and keys that are seen, of one head."""
+    t, w, docs = case["tokens"], case["window"] or case["tokens"], _doc_ids(case)
+    starts = {}
+    total = 0
+    for i, d in enumerate(docs):
+        a = starts.setdefault(d, i)
+        total += min(i - a + 1, w)
+    if case["prefix"]:
+        ends = {}
+        for i, d in enumerate(docs):
+            ends[d] = i
+        p = min(case["prefix"], t)
+        for i, d in enumerate(docs):
+            a, e = starts[d], ends[d]
+            lo = max(a, i - w + 1)
+            total += max(0, min(p, e + 1) - (i + 1)) + max(0, min(p, lo) - a)
+    return total
+
+
+def work(case):
+    c, kind = case, case["kind"]
+    if kind == "rotary":
+        values = c["batch"] * c["tokens"] * (c["heads"] + c["rows"]) * c["dim"]
+        return {"bytes": 2 * values * BYTES[c["dtype"]], "flops": 6 * values // 2}
+    if kind == "append":
+        total = sum(_fresh(c))
+        read = total * (c["heads"] + 2 * c["rows"]) * c["dim"] * BYTES[c["dtype"]]
+        written = total * c["dim"] * (c["heads"] * BYTES[c["dtype"]] + 2 * c["rows"] * BYTES[c["cache"]])
+        return {"bytes": read + written, "flops": 3 * total * (c["heads"] + c["rows"]) * c["dim"]}
+    if kind == "paged":
+        tokens = 0
+        for i, n in enumerate(_lens(c)):
+            seen = n
+            if c["window"] and c["window"] < n:
+                first = ((c["prefix"] * (i + 1)) // c["seqs"]) if c["prefix"] else 0
+                seen = min(n, c["window"] + min(first, n - c["window"]))
+            tokens += int(seen * (1.0 - c["evict"]))
+        tokens = max(1, tokens)
+        io = 2 * c["seqs"] * c["heads"] * c["dim"] * BYTES[c["dtype"]]
+        return {"bytes": 2 * tokens * c["rows"] * c["dim"] * BYTES[c["cache"]] + io,
+                "flops": 4 * tokens * c["heads"] * c["dim"]}
+    if kind == "prompt":
+        values = c["batch"] * c["tokens"] * (2 * c["heads"] + 2 * c["rows"]) * c["dim"]
+        return {"bytes": values * BYTES[c["dtype"]], "flops": 4 * c["batch"] * c["heads"] * c["dim"] * _seen_pairs(c)}
+    lens, page = _lens(c), c["page"]
+    held = sum(-(-n // page) for n in lens)
+    if kind == "fork":
+        parents = _parents(c)
+        children = [p for p in parents if p >= 0]
+        again = [p for i, p in enumerate(children) if p in children[:i]]
+        tokens = sum(lens[p] % page for p in again)
+        pages = sum(-(-(lens[p] + c["fresh"]) // page) for p in children)
+        blocks = held + c["seqs"] * (1 + -(-c["fresh"] // page))
+        return {"bytes": 4 * tokens * c["layers"] * c["rows"] * c["dim"] * BYTES[c["cache"]] + 4 * (held + pages) + 8 * blocks,
+                "flops": 0}
+    return {"bytes": 4 * held + int(4 * held * (1.0 - c["evict"])) + 8 * (held + 8) + c["rows"] * held * page // TILE, "flops": 0}
+
+
+# ---------------------------------------------------------------- in 64 bits
+
+def _exact_turn(x, positions, c):
+    """x (tokens, heads, dim) float64, a pair at a time by its complex product."""
+    x = x.clone()
+    h = c["turned"] // 2
+    pair = torch.arange(h, device=DEV)
+    one, two = (pair, pair + h) if c["layout"] == "half" else (2 * pair, 2 * pair + 1)
+    angle = positions.double()[:, None, None] * _frequencies(c["turned"])
+    z = torch.complex(x[:, :, one], x[:, :, two]) * torch.polar(torch.ones_like(angle), -angle if c.get("backward") else angle)
+    x[:, :, one], x[:, :, two] = z.real, z.imag
+    return x
+
+
+def _exact_rows(q, k, v, c, slopes, first, seen_of):
+    """Attention of q (queries, dim) of one head at places first, first + 1, ... over k, v (tokens, dim)."""
+    i = torch.arange(first, first + q.shape[0], device=DEV)[:, None]
+    j = torch.arange(k.shape[0], device=DEV)[None, :]
+    z = (q @ k.T) * c["dim"] ** -0.5
+    if c["cap"]:
+        z = c["cap"] * torch.tanh(z / c["cap"])
+    if slopes is not None:
+        z = z - slopes.double() * (i - j).abs()
+    z = torch.where(seen_of(i, j), z, -math.inf)
+    w = torch.nan_to_num(torch.softmax(z, -1), nan=0.0)
+    return w @ v
+
+
+def exact(case, seed):
+    c, kind = case, case["kind"]
+    if kind in ("fork", "evict"):
+        return None  # whole numbers, and values that are copied
+    s = prepare(case, seed)
+    if kind == "rotary":
+        return [torch.stack([_exact_turn(x.transpose(0, 1).double(), s["positions"], c).transpose(0, 1) for x in s[i]])
+                for i in ("q", "k")]
+    if kind == "append":
+        q, k = (_exact_turn(s[i].double(), s["positions"], c) for i in ("q", "k"))
+        kc, vc = s["k_cache"].double(), s["v_cache"].double()
+        tables, lens, row = s["tables"].tolist(), s["lens"].tolist(), 0
+        where = []
+        for b, n in enumerate(_fresh(c)):
+            where += [(tables[b][(lens[b] + i) // c["page"]], (lens[b] + i) % c["page"]) for i in range(n)]
+        page, slot = (torch.tensor(x, device=DEV) for x in zip(*where))
+        kc[page, :, slot] = k / s["k_scale"]
+        vc[page, :, slot] = s["v"].double() / s["v_scale"]
+        return {"q": q, "k_cache": kc, "v_cache": vc}
+    group = c["heads"] // c["rows"]
+    if kind == "paged":
+        out = torch.zeros(s["q"].shape, dtype=torch.float64, device=DEV)
+        for b, n in enumerate(s["lens"].tolist()):
+            ids = s["tables"][b, :-(-n // c["page"])].long()
+            for r in range(c["rows"]):
+                k, v = ((s[x].view(torch.uint8) if s[x].element_size() == 1 else s[x])[ids, r].view(s[x].dtype).double()
+                        .reshape(-1, c["dim"])[:n] * s[y] for x, y in (("k_cache", "k_scale"), ("v_cache", "v_scale")))
+                first = 0 if s["prefix"] is None else int(s["prefix"][b])
+
+                def seen_of(i, j):
+                    ok = (i - j < c["window"]) | (j < first) if c["window"] else j >= 0
+                    if s["evict"] is not None:
+                        whole = j // TILE < n // TILE
+                        ok = ok & ~(s["evict"][b, r][(j // TILE).clamp(max=s["evict"].shape[2] - 1)] & whole)
+                    return ok
+                for h in range(r * group, (r + 1) * group):
+                    slope = None if s["slopes"] is None else s["slopes"][h]
+                    out[b, h] = _exact_rows(s["q"][b, h:h + 1].double(), k, v, c, slope, n - 1, seen_of)[0]
+        return out
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device=DEV)
+    for b in range(c["batch"]):
+        first = 0 if s["prefix"] is None else int(s["prefix"][b])
+
+        def seen_of(i, j):
+            ok = (j <= i) & (i - j < (c["window"] or c["tokens"])) | (j < first)
+            return ok if s["docs"] is None else ok & (s["docs"][b][i] == s["docs"][b][j])
+        for h in range(c["heads"]):
+            slope = None if s["slopes"] is None else s["slopes"][h]
+            out[b, h] = _exact_rows(s["q"][b, h].double(), s["k"][b, h // group].double(), s["v"][b, h // group].double(),
+                                    c, slope, 0, seen_of)
+    return out
