@@ -1,0 +1,581 @@
+// Attention of whole prompts with changed scores (declared in
+// include/orthocache_paged.h): capped by a tanh, biased by distance, in a
+// window, behind a prefix, between documents.
+//
+// The tile step is the prefill kernel's (oc_prefill_tiles.h): a workgroup of
+// eight waves, 16 queries each, walks the 64-token tiles that any of its 128
+// queries sees, through a bit word of 64 tiles at a time.  A tile that every
+// query of a wave sees whole takes no mask; only the tiles at the borders of
+// the causal triangle, the window, the prefix and the documents do.
+//
+// What is not seen must have no effect, NaN and infinities among it.  A masked
+// score is replaced, so K needs nothing; V does, since 0 * NaN is NaN: the
+// threads that stage a border tile look at the 16-byte pieces they staged, and
+// a tile that holds a value which is not finite takes a slower p.V
+// (prompt_pv_any).
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "oc_kernels.h"
+#include "oc_paged.h"
+#include "oc_prefill_tiles.h"
+#include "oc_status.h"
+#include "orthocache_hip.h"
+#include "orthocache_paged.h"
+
+namespace oc {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+// the reference that a row's sums are relative to before its first score: below every finite score
+constexpr float kNoScore = -3e38f;
+
+struct PromptArgs {
+  const char *q, *k, *v;
+  char* out;
+  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, o_sb, o_sh, o_ss;  // bytes
+  int32_t B, Hq, Hkv, G, Sq, Skv, T, qblocks;  // T: full tiles that the evict mask covers
+  const int32_t* docs;
+  int64_t docs_sb;
+  const int2* ranges;  // (B, tiles) smallest and largest document of each tile
+  const float* slopes;
+  const int32_t* prefix;
+  const uint8_t* evict;
+  int64_t e_sb, e_sh;
+  float scale, cap;
+  int32_t window;
+  int32_t o_vec;  // out rows 8-byte aligned
+};
+
+// the smallest and largest document of each 64-token tile: one wave a tile
+__global__ __launch_bounds__(256) void doc_range_kernel(const int32_t* docs, int64_t docs_sb, int n, int tiles, int all,
+                                                        int2* out) {
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (w >= all) return;
+  const int b = w / tiles, t = w - b * tiles;
+  const int j = min(64 * t + lane, n - 1);
+  int lo = docs[b * docs_sb + j], hi = lo;
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 64));
+    hi = max(hi, __shfl_xor(hi, o, 64));
+  }
+  if (lane == 0) out[w] = int2{lo, hi};
+}
+
+// What the wave's queries see: query x is at place w_lo + x.
+struct Sight {
+  int w_lo, window, prefix;  // window: INT_MAX without one
+  const int* qdoc;           // LDS: documents of the wave's 16 queries, or null
+  const int* tdoc;           // LDS: documents of the tile's 64 tokens
+};
+
+// Online-softmax update of one tile (as pf_softmax) with the scores changed:
+// c becomes 2^(z - m) for the tokens seen, 0 for the others.  CAP:
+// z = cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)).
+template <int DT, int D, bool CAP, bool BIAS>
+__device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16], f32x4 (&c)[4], float scale, float cap,
+                                               float slope2, const Sight& e, int tok0, bool full) {
+  float mt = -__builtin_inff();
+  // the lane's place in the tile, formed from the thread index (lane =
+  // threadIdx.x mod 64) so that nothing of it is kept across the tile loop
+  int tx = threadIdx.x;
+  asm volatile("" : "+v"(tx));
+  const int r4 = (tx >> 2) & 12, x = tx & 15;
+  const int rel = e.w_lo + x - tok0 - r4;  // distance of the lane's query to its first token of the tile
+  const float d0 = (float)rel;
+  const int pre = e.prefix - tok0 - r4;
+  int doc = 0;
+  if (e.qdoc && !full) doc = e.qdoc[x];
+#pragma unroll
+  for (int tb = 0; tb < 4; ++tb) {
+    int4 td = {0, 0, 0, 0};
+    if (e.qdoc && !full) td = *reinterpret_cast<const int4*>(e.tdoc + 16 * tb + r4);
+    const int tdv[4] = {td.x, td.y, td.z, td.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float z;
+      if constexpr (CAP) {
+        if constexpr (DT == OC_F32) {
+          z = cap * kLog2e * tanhf(c[tb][i] * scale / cap);
+        } else {
+          const float ex = __builtin_amdgcn_exp2f(c[tb][i] * (2.f * kLog2e * scale / cap));
+          z = __builtin_fmaf(-2.f * kLog2e * cap, __builtin_amdgcn_rcpf(1.f + ex), kLog2e * cap);
+        }
+      } else {
+        z = c[tb][i] * (scale * kLog2e);
+      }
+      if constexpr (BIAS) z = __builtin_fmaf(-slope2, fabsf(d0 - (float)(16 * tb + i)), z);
+      if (!full) {
+        const int d = rel - (16 * tb + i);
+        const bool ok = ((d >= 0 && d < e.window) || 16 * tb + i < pre) && tdv[i] == doc && doc >= 0;
+        z = ok ? z : -__builtin_inff();
+      }
+      c[tb][i] = z;
+      mt = fmaxf(mt, z);
+    }
+  }
+  mt = fmaxf(mt, xpair<16>(mt));
+  mt = fmaxf(mt, xpair<32>(mt));
+  const bool move = mt > st.m + kPfSlack;
+  if (__builtin_amdgcn_ballot_w64(move)) {
+    const float mn = move ? mt : st.m;
+    const float alpha = __builtin_amdgcn_exp2f(st.m - mn);
+    st.m = mn;
+    st.l *= alpha;
+#pragma unroll
+    for (int nc = 0; nc < D / 16; ++nc) acc[nc] *= alpha;
+  }
+  float ls = 0.f;
+#pragma unroll
+  for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = __builtin_amdgcn_exp2f(c[tb][i] - st.m);
+      ls += p;
+      c[tb][i] = p;
+    }
+  st.l += ls;
+}
+
+// one word of V (two 16-bit values, or a float32) split: its finite values (0
+// in place of the others), and 1 where it is +inf or NaN, or -inf or NaN
+template <int DT>
+__device__ __forceinline__ void split_word(uint32_t w, uint32_t& fin, uint32_t& plus, uint32_t& minus) {
+  if constexpr (DT == OC_F32) {
+    const bool odd = (w & 0x7F800000u) == 0x7F800000u, nan = odd && (w << 9) != 0;
+    fin = odd ? 0u : w;
+    plus = odd && (nan || !(w >> 31)) ? 0x3F800000u : 0u;
+    minus = odd && (nan || w >> 31) ? 0x3F800000u : 0u;
+  } else {
+    constexpr uint32_t E = DT == OC_BF16 ? 0x7F80u : 0x7C00u, ONE = DT == OC_BF16 ? 0x3F80u : 0x3C00u;
+    fin = plus = minus = 0u;
+#pragma unroll
+    for (int k = 0; k < 32; k += 16) {
+      const uint32_t v = (w >> k) & 0xFFFFu;
+      const bool odd = (v & E) == E, nan = odd && (v & 0x7FFFu) != E;
+      fin |= (odd ? 0u : v) << k;
+      plus |= (odd && (nan || !(v >> 15)) ? ONE : 0u) << k;
+      minus |= (odd && (nan || v >> 15) ? ONE : 0u) << k;
+    }
+  }
+}
+
+// pf_pv of a tile whose V holds infinities or NaN: a token of probability 0
+// adds nothing, whatever its V.  The finite values are multiplied as ever; the
+// same products with 1 in the place of what is not finite say which outputs
+// have such a token among those of probability above 0, and get the infinity
+// (two of different sign, or a NaN: NaN).
+template <int DT, int D>
+__device__ __forceinline__ void prompt_pv_any(f32x4 (&acc)[D / 16], const f32x4 (&c)[4], const char* svb, int lane) {
+  const float inf = __builtin_inff();
+#pragma unroll
+  for (int nc = 0; nc < D / 16; ++nc) {
+    int ln = lane;  // addresses formed here, not kept in registers over the column blocks
+    asm volatile("" : "+v"(ln));
+    const int x = ln & 15, kg = ln >> 4;
+    f32x4 up = {0.f, 0.f, 0.f, 0.f}, down = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (DT == OC_F32) {
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(svb)[(16 * tb + 4 * kg + i) * D + 16 * nc + x];
+          uint32_t fin, plus, minus;
+          split_word<DT>(w, fin, plus, minus);
+          acc[nc] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(fin), c[tb][i], acc[nc], 0, 0, 0);
+          up = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(plus), c[tb][i], up, 0, 0, 0);
+          down = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(minus), c[tb][i], down, 0, 0, 0);
+        }
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // operands as in pf_pv
+        uint32_t p[4], fin[4], plus[4], minus[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = pf_pack<DT>(c[2 * j + e / 2][2 * (e % 2)], c[2 * j + e / 2][2 * (e % 2) + 1]);
+        const int vrow = 32 * j + 8 * kg + (x >> 2);
+        const uint16_t* rowp = reinterpret_cast<const uint16_t*>(svb) + vrow * D + 4 * (x & 3) +
+                               16 * (nc ^ PfTile<DT, D>::vswz(vrow));
+        const u32x2 w0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                       (__attribute__((address_space(3))) s16x4*)rowp));
+        const u32x2 w1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                       (__attribute__((address_space(3))) s16x4*)(rowp + 4 * D)));
+        split_word<DT>(w0[0], fin[0], plus[0], minus[0]);
+        split_word<DT>(w0[1], fin[1], plus[1], minus[1]);
+        split_word<DT>(w1[0], fin[2], plus[2], minus[2]);
+        split_word<DT>(w1[1], fin[3], plus[3], minus[3]);
+        acc[nc] = mfma_qk<DT>(fin, p, acc[nc]);
+        up = mfma_qk<DT>(plus, p, up);
+        down = mfma_qk<DT>(minus, p, down);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc[nc][u] += up[u] > 0.f ? inf : 0.f;
+      acc[nc][u] -= down[u] > 0.f ? inf : 0.f;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // one column block at a time in registers
+  }
+}
+
+// whether one of 16 bytes of type DT is infinite or NaN
+template <int DT>
+__device__ __forceinline__ bool not_finite(const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  constexpr uint32_t E = DT == OC_F32 ? 0x7F800000u : (DT == OC_BF16 ? 0x7F80u : 0x7C00u);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    bad |= (w[i] & E) == E;
+    if constexpr (DT != OC_F32) bad |= (w[i] >> 16 & E) == E;
+  }
+  return bad;
+}
+
+__device__ __forceinline__ int wave_min_i(int v) {
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+template <int DT, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT == OC_F32 && D == 128 ? 1 : 4))) void prompt_kernel(
+    const PromptArgs a) {
+  using L = PfTile<DT, D>;
+  __shared__ __attribute__((aligned(16))) char sh[L::LDS];
+  __shared__ __attribute__((aligned(16))) int sdoc[2][64];
+  __shared__ int sqdoc[kPfRows];
+  __shared__ int bad_tile[2];  // the tile of each stage that holds V values which are not finite
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = tid >> 6;
+  // (batch, head) pairs and query blocks as in the prefill kernel: an eighth
+  // of the pairs per XCD, longest causal windows first
+  const int nbh = a.B * a.Hq;
+  const int i = blockIdx.x;
+  int bh, e;
+  if (nbh % 8 == 0) {
+    const int hpx = nbh / 8, j = i / 8;
+    bh = (i % 8) * hpx + j % hpx;
+    e = j / hpx;
+  } else {
+    bh = i % nbh;
+    e = i / nbh;
+  }
+  const int qb = a.qblocks - 1 - e;
+  const int b = bh / a.Hq;
+  const int h = bh % a.Hq;
+  const int kv = h / a.G;
+  const int pos0 = qb * kPfRows + 16 * wave;
+  const int off = a.Skv - a.Sq;
+  const int x = lane & 15;
+  const int window = a.window > 0 ? a.window : INT_MAX;
+  const int prefix = a.prefix ? min(max(a.prefix[b], 0), a.Skv) : 0;
+  const int32_t* docs = a.docs ? a.docs + b * a.docs_sb : nullptr;
+  auto doc_at = [&](int s) {  // the document of query s, -1 for none
+    const int p = s + off;
+    return s < a.Sq && p >= 0 ? docs[p] : -1;
+  };
+  // documents of the wave's queries, and of the workgroup's: [least, most] of those that are not negative
+  int wd0 = 0, wd1 = 0, gd0 = 0, gd1 = 0;
+  if (docs) {
+    const int doc = doc_at(pos0 + x);
+    if (lane < 16) sqdoc[16 * wave + lane] = doc;  // read by this wave alone
+    const int d0 = doc_at(qb * kPfRows + lane), d1 = doc_at(qb * kPfRows + 64 + lane);
+    auto least = [](int d) { return d < 0 ? INT_MAX : d; };
+    wd0 = wave_min_i(least(doc)), wd1 = wave_max_i(doc);
+    // (a wave with a query past Sq or of no document is not uniform)
+    if (__builtin_amdgcn_ballot_w64(doc < 0 && pos0 + x < a.Sq)) wd1 = INT_MAX;
+    gd0 = wave_min_i(min(least(d0), least(d1))), gd1 = wave_max_i(max(d0, d1));
+  }
+  const int2* ranges = a.docs ? a.ranges + (int64_t)b * ((a.Skv + 63) / 64) : nullptr;
+  // places of the wave's first and last query, and of the workgroup's
+  const int w_lo = pos0 + off, w_hi = min(pos0 + 15, a.Sq - 1) + off;
+  const int g_lo = qb * kPfRows + off, g_hi = min(qb * kPfRows + kPfRows - 1, a.Sq - 1) + off;
+  auto needed = [&](int t, int lo, int hi) {  // whether queries at places lo .. hi see a token of tile t
+    return (64 * t <= hi && (window == INT_MAX || 64 * t + 63 > lo - window)) || 64 * t < prefix;
+  };
+  auto whole = [&](int t, int lo, int hi) {  // whether they all see all of it (documents apart)
+    return 64 * t + 63 < a.Skv &&
+           ((64 * t + 63 <= lo && (window == INT_MAX || hi - 64 * t < window)) || 64 * t + 63 < prefix);
+  };
+  const int t_hi = (min(max(max(g_hi + 1, prefix), 0), a.Skv) + 63) / 64;
+  const bool active = pos0 < a.Sq;
+
+  PrefillArgs pa;  // what the tile staging and the q load read
+  pa.q_ss = a.q_ss, pa.Sq = a.Sq, pa.Skv = a.Skv, pa.k_ss = a.k_ss, pa.v_ss = a.v_ss;
+  PfQ<DT, D> q;
+  pf_load_q<DT, D>(pa, a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh, pos0, lane, q);
+  const char* kh = a.k + (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh;
+  const char* vh = a.v + (int64_t)b * a.v_sb + (int64_t)kv * a.v_sh;
+  const uint8_t* erow = a.evict ? a.evict + (int64_t)b * a.e_sb + (int64_t)kv * a.e_sh : nullptr;
+  const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+
+  // the tiles of the workgroup, 64 at a time; of those, the ones whose
+  // documents are all the wave's one document
+  int word = 0;
+  uint64_t bits = 0, ubits = 0;
+  auto load_word = [&](int w) {
+    const int t = 64 * w + (int)__lane_id();
+    bool keep = t < t_hi && needed(t, g_lo, g_hi);
+    if (erow) keep = keep && !(t < a.T && erow[min(t, a.T - 1)]);
+    bool one = true;
+    if (docs) {
+      const int2 d = ranges[min(t, (a.Skv - 1) / 64)];
+      keep = keep && d.y >= gd0 && d.x <= gd1;
+      one = d.x == d.y && d.x == wd0 && d.x == wd1;
+    }
+    bits = __builtin_amdgcn_ballot_w64(keep);
+    ubits = __builtin_amdgcn_ballot_w64(one);
+  };
+  bool uniform = true;  // of the tile last taken
+  auto next_tile = [&]() {
+    while (bits == 0) {
+      if (64 * ++word >= t_hi) return t_hi;
+      load_word(word);
+    }
+    const int t = 64 * word + __builtin_ctzll(bits);
+    uniform = ubits & bits & -bits;
+    bits &= bits - 1;
+    return t;
+  };
+  PfState st;
+  f32x4 accp[D / 16];
+  auto stage_k = [&](int s) { return sh + s * 2 * L::KV; };
+  auto stage_v = [&](int s) { return sh + s * 2 * L::KV + L::KV; };
+  auto border = [&](int t) { return docs || !whole(t, g_lo, g_hi); };  // uniform over the workgroup
+  // One pass over the tiles.  The first takes V to be finite where it matters
+  // and gives up (true) at the first border tile whose V is not; the second
+  // then starts over with prompt_pv_any.  (Both forms of p.V in one loop need
+  // more registers than two workgroups a CU leave.)
+  auto pass = [&](auto any_c) -> bool {
+    constexpr bool ANY = decltype(any_c)::value;
+    word = 0;
+    bits = ubits = 0;
+    if (t_hi > 0) load_word(0);
+    st = PfState{kNoScore, 0.f, 0.f, 0};
+#pragma unroll
+    for (int nc = 0; nc < D / 16; ++nc) accp[nc] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (tid < 2) bad_tile[tid] = -1;
+    auto compute = [&](int t, bool uni, const char* __restrict__ ck, const char* __restrict__ cv,
+                       const int* __restrict__ cd) {
+      if (!active || !needed(t, w_lo, w_hi)) return;
+      const bool full = uni && whole(t, w_lo, w_hi);
+      f32x4 c[4];
+      pf_logits<DT, D>(q, ck, lane, c);
+      const Sight eye{w_lo, window, prefix, docs ? sqdoc + 16 * wave : nullptr, cd};
+      prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, a.scale, a.cap, slope2, eye, t * 64, full);
+      if constexpr (ANY) prompt_pv_any<DT, D>(accp, c, cv, lane);
+      else pf_pv<DT, D, false>(accp, c, cv, lane);
+    };
+    int t = next_tile();
+    bool uni = uniform;
+    __syncthreads();  // bad_tile
+    if constexpr (L::STAGES == 2) {
+      // the tile's documents go straight to LDS as well (past the last: 0, masked as no one sees those)
+      auto fetch = [&](int t, char* nk, char* nv, int* nd) {
+        pf_fetch_lds<DT, D>(pa, kh, vh, t, tid, nk, nv);
+        if (docs && wave == 0) {
+          const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)pf_uniform((const char*)docs), (short)0, __builtin_amdgcn_readfirstlane(a.Skv * 4), 0x00020000);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)nd, 4, 4 * (64 * t + lane),
+                                                   0, 0, 0);
+        }
+      };
+      // what this thread staged of tile t's V, looked at once its loads have landed
+      auto landed = [&](int t, int s) {
+        if (ANY || !border(t)) return;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < L::NL; ++j)
+          bad |= not_finite<DT>(*reinterpret_cast<const uint4*>(stage_v(s) + 16 * (tid + kPfThreads * j)));
+        if (bad) bad_tile[s] = t;
+      };
+      if (t < t_hi) fetch(t, stage_k(0), stage_v(0), sdoc[0]);
+      __builtin_amdgcn_s_waitcnt(0);
+      if (t < t_hi) landed(t, 0);
+      int s = 0;
+      // the stages are restrict parameters, as in the prefill kernel: no wait for
+      // the loads into one before the reads of the other
+      auto step = [&](int tn, char* __restrict__ nk, char* __restrict__ nv, int* __restrict__ nd,
+                      const char* __restrict__ ck, const char* __restrict__ cv, const int* __restrict__ cd) {
+        if (tn < t_hi) fetch(tn, nk, nv, nd);
+        compute(t, uni, ck, cv, cd);
+      };
+      while (t < t_hi) {
+        __syncthreads();  // stage s is complete; every wave is done with stage s ^ 1
+        if (!ANY && bad_tile[s] == t) return true;  // (uniform; no load is in flight)
+        const int tn = next_tile();
+        const bool un = uniform;
+        step(tn, stage_k(1 - s), stage_v(1 - s), sdoc[1 - s], stage_k(s), stage_v(s), sdoc[s]);
+        __builtin_amdgcn_s_waitcnt(0);
+        s = 1 - s;
+        if (tn < t_hi) landed(tn, s);
+        t = tn;
+        uni = un;
+      }
+    } else {
+      // one stage (float32, head_dim 128): the next tile waits in registers
+      PfStage<DT, D> reg;
+      int dn = 0;
+      auto fetch = [&](int t) {
+        pf_fetch<DT, D>(pa, kh, vh, t, tid, reg);
+        if (docs && wave == 0) dn = docs[min(64 * t + lane, a.Skv - 1)];
+      };
+      auto stash = [&](int t) {
+        pf_stash<DT, D>(reg, tid, stage_k(0), stage_v(0));
+        if (docs && wave == 0) sdoc[0][lane] = dn;
+        if (ANY || !border(t)) return;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < L::NL; ++j) bad |= not_finite<DT>(reg.v[j]);
+        if (bad) bad_tile[0] = t;
+      };
+      if (t < t_hi) {
+        fetch(t);
+        stash(t);
+      }
+      while (t < t_hi) {
+        __syncthreads();  // the stage is complete
+        if (!ANY && bad_tile[0] == t) return true;
+        const int tn = next_tile();
+        const bool un = uniform;
+        if (tn < t_hi) fetch(tn);  // in flight during this tile
+        compute(t, uni, stage_k(0), stage_v(0), sdoc[0]);
+        __syncthreads();  // the stage is free again
+        if (tn < t_hi) stash(tn);
+        t = tn;
+        uni = un;
+      }
+    }
+    return false;
+  };
+  if (pass(std::false_type{})) {
+    __syncthreads();  // every wave has read bad_tile
+    pass(std::true_type{});
+  }
+
+  // sums over the query's four lanes; lane 16r + x writes columns 16nc + 4r .. + 4 of query x
+  float l = st.l;
+  l += xpair<16>(l);
+  l += xpair<32>(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  int tl = threadIdx.x;  // formed after the loop, as in the prefill kernel
+  asm volatile("" : "+v"(tl));
+  const int qpos = pos0 + (tl & 15), r = (tl >> 4) & 3;
+  if (qpos < a.Sq) {
+    char* orow = a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qpos * a.o_ss;
+#pragma unroll
+    for (int nc = 0; nc < D / 16; ++nc) {
+      const int col = 16 * nc + 4 * r;
+      if constexpr (DT == OC_F32) {
+        *reinterpret_cast<float4*>(orow + 4 * col) =
+            float4{accp[nc][0] * inv, accp[nc][1] * inv, accp[nc][2] * inv, accp[nc][3] * inv};
+      } else {
+        const uint2 w = {pf_pack<DT>(accp[nc][0] * inv, accp[nc][1] * inv),
+                         pf_pack<DT>(accp[nc][2] * inv, accp[nc][3] * inv)};
+        if (a.o_vec) {
+          *reinterpret_cast<uint2*>(orow + 2 * col) = w;
+        } else {
+          uint16_t* o = reinterpret_cast<uint16_t*>(orow + 2 * col);
+          o[0] = (uint16_t)w.x, o[1] = (uint16_t)(w.x >> 16);
+          o[2] = (uint16_t)w.y, o[3] = (uint16_t)(w.y >> 16);
+        }
+      }
+    }
+  }
+}
+
+template <int DT, int D>
+void launch_prompt(const PromptArgs& a, unsigned blocks, hipStream_t s) {
+  const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
+  auto k = cap ? (bias ? prompt_kernel<DT, D, true, true> : prompt_kernel<DT, D, true, false>)
+               : (bias ? prompt_kernel<DT, D, false, true> : prompt_kernel<DT, D, false, false>);
+  hipLaunchKernelGGL(k, dim3(blocks), dim3(kPfThreads), 0, s, a);
+}
+
+template <int DT>
+void launch_prompt_d(const PromptArgs& a, int d, unsigned blocks, hipStream_t s) {
+  if (d == 64) launch_prompt<DT, 64>(a, blocks, s);
+  else launch_prompt<DT, 128>(a, blocks, s);
+}
+
+constexpr int kMaxKv = 1 << 24;  // distances are exact in float32 up to here
+
+int check_prompt(const oc_attend_prompt_params* p) {
+  if (!p) return fail(OC_ERR_INVALID, "NULL parameters");
+  if (!paged_float(p->dtype)) return fail(OC_ERR_INVALID, "dtype %d", p->dtype);
+  if (p->head_dim != 64 && p->head_dim != 128) return fail(OC_ERR_UNSUPPORTED, "head_dim %d (64 or 128)", p->head_dim);
+  if (p->batch < 0 || p->num_q_heads < 0 || p->num_kv_heads < 0 || p->q_len < 0 || p->kv_len < 0)
+    return fail(OC_ERR_INVALID, "bad sizes");
+  if (p->num_q_heads && (!p->num_kv_heads || p->num_q_heads % p->num_kv_heads))
+    return fail(OC_ERR_INVALID, "%d query heads on %d kv heads", p->num_q_heads, p->num_kv_heads);
+  if (p->kv_len > kMaxKv || p->q_len > kMaxKv) return fail(OC_ERR_UNSUPPORTED, "over 2^24 tokens");
+  return check_mods(&p->mods);
+}
+
+}  // namespace
+}  // namespace oc
+
+using namespace oc;
+
+extern "C" size_t oc_attend_prompt_workspace_size(const oc_attend_prompt_params* p) {
+  if (check_prompt(p) != OC_OK || !p->documents) return 0;
+  return (size_t)p->batch * (size_t)((p->kv_len + 63) / 64) * sizeof(int2);
+}
+
+extern "C" int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream) {
+  if (const int rc = check_prompt(p)) return rc;
+  if (p->batch == 0 || p->num_q_heads == 0 || p->q_len == 0) return OC_OK;
+  if (!p->q || !p->out || (p->kv_len && (!p->k || !p->v))) return fail(OC_ERR_INVALID, "NULL pointer");
+  const int es = p->dtype == OC_F32 ? 4 : 2;
+  for (const void* t : {p->q, p->k, p->v})
+    if ((uintptr_t)t % 16) return fail(OC_ERR_INVALID, "q/k/v must be 16-byte aligned");
+  for (int64_t st : {p->q_stride_b, p->q_stride_h, p->q_stride_s, p->k_stride_b, p->k_stride_h, p->k_stride_s,
+                     p->v_stride_b, p->v_stride_h, p->v_stride_s})
+    if ((st * es) % 16) return fail(OC_ERR_INVALID, "q/k/v strides must be multiples of 16 bytes");
+  if (p->dtype == OC_F32)
+    for (int64_t st : {(int64_t)(uintptr_t)p->out, p->out_stride_b * es, p->out_stride_h * es, p->out_stride_s * es})
+      if (st % 16) return fail(OC_ERR_INVALID, "float32 out rows must be 16-byte aligned");
+  if (p->k_stride_s * es * 64 > 0x7FFFFFFF || p->v_stride_s * es * 64 > 0x7FFFFFFF)
+    return fail(OC_ERR_UNSUPPORTED, "token stride too large");
+  if (p->kv_len && (p->k_stride_s < p->head_dim || p->v_stride_s < p->head_dim))
+    return fail(OC_ERR_INVALID, "token stride smaller than head_dim");
+  const size_t need = oc_attend_prompt_workspace_size(p);
+  if (need && (!p->workspace || p->workspace_bytes < need))
+    return fail(OC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", p->workspace_bytes, need);
+  PromptArgs a{};
+  a.q = (const char*)p->q, a.k = (const char*)p->k, a.v = (const char*)p->v, a.out = (char*)p->out;
+  a.q_sb = p->q_stride_b * es, a.q_sh = p->q_stride_h * es, a.q_ss = p->q_stride_s * es;
+  a.k_sb = p->k_stride_b * es, a.k_sh = p->k_stride_h * es, a.k_ss = p->k_stride_s * es;
+  a.v_sb = p->v_stride_b * es, a.v_sh = p->v_stride_h * es, a.v_ss = p->v_stride_s * es;
+  a.o_sb = p->out_stride_b * es, a.o_sh = p->out_stride_h * es, a.o_ss = p->out_stride_s * es;
+  a.o_vec = ((uintptr_t)p->out | a.o_sb | a.o_sh | a.o_ss) % 8 == 0;
+  a.B = p->batch, a.Hq = p->num_q_heads, a.Hkv = p->num_kv_heads, a.G = p->num_q_heads / p->num_kv_heads;
+  a.Sq = p->q_len, a.Skv = p->kv_len, a.qblocks = (p->q_len + kPfRows - 1) / kPfRows;
+  a.T = std::min(p->kv_len / 64, p->mods.evict ? p->mods.evict_cols : 0);
+  a.docs = p->kv_len ? p->documents : nullptr, a.docs_sb = p->documents_stride_b, a.ranges = (const int2*)p->workspace;
+  a.slopes = p->mods.slopes, a.prefix = p->mods.prefix_lens;
+  a.evict = a.T > 0 ? p->mods.evict : nullptr, a.e_sb = p->mods.evict_stride_b, a.e_sh = p->mods.evict_stride_h;
+  a.scale = p->mods.scale, a.cap = p->mods.softcap, a.window = p->mods.window;
+  const int64_t blocks = (int64_t)p->batch * p->num_q_heads * a.qblocks;
+  const int64_t tiles = (int64_t)p->batch * ((p->kv_len + 63) / 64);
+  if (blocks > 0x7FFFFFFF || tiles > 0x7FFFFFFF || (int64_t)p->batch * p->num_q_heads > 0x7FFFFFFF)
+    return fail(OC_ERR_UNSUPPORTED, "too many workgroups");
+  const hipStream_t s = (hipStream_t)stream;
+  if (a.docs)
+    hipLaunchKernelGGL(doc_range_kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, s, a.docs, a.docs_sb, a.Skv,
+                       (a.Skv + 63) / 64, (int)tiles, (int2*)p->workspace);
+  if (p->dtype == OC_F32) launch_prompt_d<OC_F32>(a, p->head_dim, (unsigned)blocks, s);
+  else if (p->dtype == OC_F16) launch_prompt_d<OC_F16>(a, p->head_dim, (unsigned)blocks, s);
+  else launch_prompt_d<OC_BF16>(a, p->head_dim, (unsigned)blocks, s);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? OC_OK : hip_fail(e, "prompt launch");
+}

@@ -36,6 +36,9 @@ from .triton_kernels.paged_eviction import (  # noqa: F401
     fused_orthocache_attention_paged,
     score_paged_tiles,
 )
+from .rotary import RotaryTable, apply_rotary, rotary_table  # noqa: F401
+from .paged_cache import OutOfPages, PageTables, append_paged, evict_pages, fork_pages  # noqa: F401
+from .changed_scores import attend_paged, attend_prompt  # noqa: F401
 
 __all__ = [
     "__version__",
@@ -57,4 +60,14 @@ __all__ = [
     "fused_orthocache_attention_v3_gqa",
     "fused_orthocache_attention_paged",
     "score_paged_tiles",
+    "RotaryTable",
+    "rotary_table",
+    "apply_rotary",
+    "append_paged",
+    "PageTables",
+    "OutOfPages",
+    "fork_pages",
+    "evict_pages",
+    "attend_paged",
+    "attend_prompt",
 ]

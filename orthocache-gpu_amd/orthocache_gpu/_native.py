@@ -135,6 +135,101 @@ class OcHookDecodeParams(ctypes.Structure):
     ]
 
 
+# ---- include/orthocache_paged.h
+
+# bits of a page operator's status
+OC_PAGES_NO_ROOM, OC_PAGES_BAD_PARENT, OC_PAGES_TOO_LONG, OC_PAGES_BAD_BLOCK = 1, 2, 4, 8
+
+_f32 = ctypes.c_float
+
+
+class OcRotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("x", _p * 2), ("y", _p * 2),
+        ("x_stride_b", _i64 * 2), ("x_stride_h", _i64 * 2), ("x_stride_s", _i64 * 2),
+        ("y_stride_b", _i64 * 2), ("y_stride_h", _i64 * 2), ("y_stride_s", _i64 * 2),
+        ("heads", _i32 * 2),
+        ("dtype", _i32), ("batch", _i32), ("tokens", _i32), ("head_dim", _i32), ("rotary_dim", _i32),
+        ("interleaved", _i32), ("backward", _i32), ("positions_64", _i32),
+        ("positions", _p), ("positions_stride_b", _i64), ("inv_freq", _p), ("scale", _f32),
+    ]
+
+
+class OcAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("k", _p), ("v", _p), ("q_out", _p),
+        ("q_stride_s", _i64), ("q_stride_h", _i64), ("k_stride_s", _i64), ("k_stride_h", _i64),
+        ("v_stride_s", _i64), ("v_stride_h", _i64), ("q_out_stride_s", _i64), ("q_out_stride_h", _i64),
+        ("k_cache", _p), ("v_cache", _p),
+        ("k_cache_stride_b", _i64), ("k_cache_stride_h", _i64), ("k_cache_stride_s", _i64),
+        ("v_cache_stride_b", _i64), ("v_cache_stride_h", _i64), ("v_cache_stride_s", _i64),
+        ("dtype", _i32), ("cache_dtype", _i32),
+        ("tokens", _i32), ("num_seqs", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("block_size", _i32), ("max_blocks", _i32), ("num_blocks", _i64),
+        ("block_tables", _p), ("bt_stride", _i64), ("context_lens", _p), ("cu_seqlens", _p),
+        ("positions", _p), ("positions_64", _i32), ("interleaved", _i32), ("inv_freq", _p),
+        ("scale", _f32), ("k_scale", _f32), ("v_scale", _f32), ("error_flag", _p),
+    ]
+
+
+class OcScoreMods(ctypes.Structure):
+    _fields_ = [
+        ("scale", _f32), ("softcap", _f32), ("slopes", _p), ("prefix_lens", _p),
+        ("evict", _p), ("evict_stride_b", _i64), ("evict_stride_h", _i64), ("evict_cols", _i32), ("window", _i32),
+    ]
+
+
+class OcAttendPagedParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("q_stride_b", _i64), ("q_stride_h", _i64), ("k", _p), ("v", _p),
+        ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_s", _i64),
+        ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_s", _i64),
+        ("block_tables", _p), ("bt_stride", _i64), ("num_blocks", _i64), ("context_lens", _p),
+        ("max_blocks", _i32), ("block_size", _i32), ("dtype", _i32), ("cache_dtype", _i32),
+        ("num_seqs", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("k_scale", _f32), ("v_scale", _f32), ("mods", OcScoreMods), ("num_splits", _i32), ("portable", _i32),
+        ("out", _p), ("out_stride_b", _i64), ("out_stride_h", _i64), ("error_flag", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class OcAttendPromptParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("q_stride_b", _i64), ("q_stride_h", _i64), ("q_stride_s", _i64),
+        ("k", _p), ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_s", _i64),
+        ("v", _p), ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_s", _i64),
+        ("out", _p), ("out_stride_b", _i64), ("out_stride_h", _i64), ("out_stride_s", _i64),
+        ("dtype", _i32), ("batch", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32),
+        ("q_len", _i32), ("kv_len", _i32), ("head_dim", _i32),
+        ("documents", _p), ("documents_stride_b", _i64), ("mods", OcScoreMods),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class OcForkParams(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", _p), ("v_cache", _p),
+        ("k_stride_l", _i64), ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_s", _i64),
+        ("v_stride_l", _i64), ("v_stride_b", _i64), ("v_stride_h", _i64), ("v_stride_s", _i64),
+        ("cache_dtype", _i32), ("layers", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32),
+        ("num_seqs", _i32), ("num_children", _i32), ("max_blocks", _i32), ("out_max_blocks", _i32), ("num_blocks", _i64),
+        ("block_tables", _p), ("bt_stride", _i64), ("context_lens", _p), ("ref_counts", _p),
+        ("parents", _p), ("new_tokens", _p),
+        ("out_block_tables", _p), ("out_bt_stride", _i64), ("out_context_lens", _p), ("out_ref_counts", _p),
+        ("status", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class OcEvictParams(ctypes.Structure):
+    _fields_ = [
+        ("num_seqs", _i32), ("num_kv_heads", _i32), ("block_size", _i32), ("max_blocks", _i32), ("num_blocks", _i64),
+        ("block_tables", _p), ("bt_stride", _i64), ("context_lens", _p), ("ref_counts", _p),
+        ("evict", _p), ("evict_stride_b", _i64), ("evict_stride_h", _i64), ("evict_cols", _i32), ("tile_map_cols", _i32),
+        ("out_block_tables", _p), ("out_bt_stride", _i64), ("out_context_lens", _p), ("out_ref_counts", _p),
+        ("tile_map", _p), ("status", _p),
+    ]
+
+
 class OcDeviceInfo(ctypes.Structure):
     _fields_ = [
         ("arch", ctypes.c_char * 64), ("name", ctypes.c_char * 128), ("compute_units", _i32), ("wave_size", _i32),
@@ -143,7 +238,7 @@ class OcDeviceInfo(ctypes.Structure):
     ]
 
 
-# every function declared in include/orthocache_hip.h: name -> (restype, argtypes)
+# every function declared in include/orthocache_hip.h and orthocache_paged.h: name -> (restype, argtypes)
 SIGNATURES = {
     "oc_score_tiles": (_i32, [ctypes.POINTER(OcKvDesc), ctypes.c_double, _p, _p, _p, _p, _i64, _p]),
     "oc_fwht_tiles": (_i32, [ctypes.POINTER(OcKvDesc), _p, _p]),
@@ -190,6 +285,16 @@ SIGNATURES = {
     "oc_abi_sizes": (_i32, [ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
     "oc_device_cu_count": (_i32, [ctypes.POINTER(_i32)]),
     "oc_device_props": (_i32, [ctypes.POINTER(OcDeviceInfo)]),
+    "oc_apply_rotary": (_i32, [ctypes.POINTER(OcRotaryParams), _p]),
+    "oc_append_paged": (_i32, [ctypes.POINTER(OcAppendParams), _p]),
+    "oc_attend_paged": (_i32, [ctypes.POINTER(OcAttendPagedParams), _p]),
+    "oc_attend_paged_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(OcAttendPagedParams)]),
+    "oc_attend_prompt": (_i32, [ctypes.POINTER(OcAttendPromptParams), _p]),
+    "oc_attend_prompt_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(OcAttendPromptParams)]),
+    "oc_fork_pages": (_i32, [ctypes.POINTER(OcForkParams), _p]),
+    "oc_fork_pages_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(OcForkParams)]),
+    "oc_evict_pages": (_i32, [ctypes.POINTER(OcEvictParams), _p]),
+    "oc_paged_params_bytes": (None, [ctypes.POINTER(ctypes.c_size_t)]),
     "oc_version": (ctypes.c_char_p, []),
     "oc_last_error": (ctypes.c_char_p, []),
 }
@@ -236,6 +341,13 @@ def lib():
                            ("oc_spectra_params_bytes", OcSpectraParams),
                            ("oc_hook_decode_params_bytes", OcHookDecodeParams)):
                 if getattr(handle, fn)() != ctypes.sizeof(st):
+                    raise RuntimeError(f"orthocache_gpu: {st.__name__} layout mismatch between the binding and "
+                                       f"{LIB_PATH}")
+            sizes = (ctypes.c_size_t * 6)()
+            handle.oc_paged_params_bytes(sizes)
+            for sz, st in zip(sizes, (OcRotaryParams, OcAppendParams, OcAttendPagedParams, OcAttendPromptParams,
+                                      OcForkParams, OcEvictParams)):
+                if sz != ctypes.sizeof(st):
                     raise RuntimeError(f"orthocache_gpu: {st.__name__} layout mismatch between the binding and "
                                        f"{LIB_PATH}")
             _lib = handle
