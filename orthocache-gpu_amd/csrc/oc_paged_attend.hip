@@ -236,6 +236,342 @@ __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const Page
   }
 }
 
+// ------------------------------------------------------------ matrix cores
+//
+// 16-bit queries over a 16-bit or fp8 cache, head_dim 64, 128 or 256, blocks of
+// 8 tokens or more.  A workgroup of four waves takes a share of one (sequence,
+// kv head) for up to 16 query heads; a wave takes units of 32 tokens, K and V in
+// registers, and asks for the next unit's K as soon as the scores have used this
+// one's, for its V as soon as p.V has.  Nothing but the block ids goes through
+// LDS:
+//
+//   S^T = K q^T, K as the A operand: row 4r + i of instruction tb is token 8r +
+//   4tb + i, so lane (r, head) ends up with the scores of tokens 8r .. 8r + 7.
+//   O^T += V^T P^T, V^T as the A operand: lane (kg, x) loads columns 8x .. 8x +
+//   7 (4x .. at head_dim 64) of the tokens 8kg .. 8kg + 7, a whole row per 16
+//   lanes, and instruction nc takes column 8x + nc of its eight tokens: the 8x8
+//   block is turned in registers by one v_perm per two values.  P^T, the B
+//   operand, is the lane's own eight probabilities.
+//
+// Bound by the bytes of K and V: a unit of 32 tokens of 128 columns is 16 KiB
+// of loads to about 500 cycles of work.
+
+constexpr int kPmWaves = 4;
+constexpr int kPmThreads = kPmWaves * kWave;
+constexpr int kPmHeads = 16;
+constexpr int kPmUnit = 32;
+constexpr int kPmPages = kPmUnit / 8;  // blocks that a unit may touch
+
+template <int CT, int D>
+struct PmBuf {
+  static constexpr bool F8 = CT == OC_FP8_E4M3FN;
+  static constexpr int KW = D / 32 * (F8 ? 2 : 4);  // words of a token's K in a lane (its quarter of the columns)
+  static constexpr int CPL = D == 64 ? 4 : 8;       // V columns of a lane's chunk
+  static constexpr int CH = D / (16 * CPL);         // chunks of a lane
+  static constexpr int VW = CPL * (F8 ? 1 : 2) / 4; // words of a chunk
+  uint32_t k[2][KW];
+  uint32_t v[8][CH][VW];
+};
+
+template <int W>
+__device__ __forceinline__ void pm_load(const char* p, uint32_t* w) {
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+  if constexpr (W == 4) {
+    const v4u u = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p));
+    w[0] = u[0], w[1] = u[1], w[2] = u[2], w[3] = u[3];
+  } else if constexpr (W == 2) {
+    const v2u u = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(p));
+    w[0] = u[0], w[1] = u[1];
+  } else {
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+// two fp8 values (half h of word w) as a pair of the 16-bit type MT, exactly
+template <int MT>
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool high) {
+  if constexpr (MT == OC_BF16)
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  else
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+}
+
+template <int MT>
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {
+  if constexpr (MT == OC_BF16) return bf16_bits(lo) | (bf16_bits(hi) << 16);
+  else
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) |
+           ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
+}
+
+template <int CT, int MT, int D>
+__global__ __launch_bounds__(kPmThreads) __attribute__((amdgpu_waves_per_eu(D == 256 && CT != OC_FP8_E4M3FN ? 1 : 2))) void paged_mfma_kernel(
+    const PagedArgs a) {
+  using B = PmBuf<CT, D>;
+  constexpr bool F8 = B::F8;
+  constexpr int ES = F8 ? 1 : 2;
+  __shared__ int sid[kPmWaves][kWave][kPmPages];
+  __shared__ float sacc[kPmWaves][kPmHeads][D + 4];
+  __shared__ float sm[kPmWaves][kPmHeads], sl[kPmWaves][kPmHeads];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int x = lane & 15, r = lane >> 4;
+  const int chunks = (a.G + kPmHeads - 1) / kPmHeads;
+  const int b = blockIdx.z, kv = blockIdx.y / chunks, split = blockIdx.x;
+  const int g0 = (blockIdx.y % chunks) * kPmHeads;
+  const int ng = min(kPmHeads, a.G - g0);
+  const int h0 = kv * a.G + g0;
+  const Seen s = seen_of(a, b);
+  // q as the B operand: lane (kg = r, head x), columns q_col(kg, dc) .. + 8 for instruction dc
+  uint32_t q[D / 32][4];
+#pragma unroll
+  for (int dc = 0; dc < D / 32; ++dc) {
+    uint4 u = {0u, 0u, 0u, 0u};
+    if (x < ng) u = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (h0 + x) * a.q_sh + 2 * q_col<F8>(r, dc));
+    q[dc][0] = u.x, q[dc][1] = u.y, q[dc][2] = u.z, q[dc][3] = u.w;
+  }
+  const float slope2 = a.slopes && x < ng ? a.slopes[h0 + x] * kLog2e : 0.f;
+  const bool capped = a.cap > 0.f;
+  // capped: z = cap - 2 cap / (1 + e^(2 s / cap)), all in base-2 units
+  const float ex2 = capped ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+  const float cap2 = a.cap * kLog2e;
+
+  const int32_t* row = a.tables + b * a.bt_stride;
+  const uint8_t* ev = a.evict ? a.evict + b * a.e_sb + kv * a.e_sh : nullptr;
+  const int bs = 1 << a.block_log2;
+  const int64_t all = 2 * (int64_t)s.count();
+  const int lo = (int)(all * split / a.P), hi = (int)(all * (split + 1) / a.P);
+
+  // The wave's units lo + wave, + 4, ...: 64 at a time, a lane each finds its
+  // unit's first token, whether anything of it is seen, and its block ids.
+  int word = 0, first_tok = 0;  // first_tok: of this lane's unit of the word
+  uint64_t bits = 0;
+  auto load_word = [&]() {
+    const int64_t i = lo + wave + (int64_t)kPmWaves * (64 * word + lane);
+    bool keep = i < hi;
+    int t0 = 0;
+    if (keep) {
+      const int t = s.tile((int)(i >> 1));
+      t0 = 64 * t + 32 * (int)(i & 1);
+      auto seen = [&](int from, int to) {  // any of the tokens from .. to - 1
+        return from < s.L && (s.L - min(to, s.L) < a.window || from < s.prefix);
+      };
+      keep = seen(t0, t0 + kPmUnit) && !(ev && t < a.e_cols && t < s.L / 64 && ev[t]);
+      if (keep) {
+        const int step = min(bs, kPmUnit);
+        int id = -1;
+        for (int p = 0; p < kPmPages; ++p) {
+          const int from = t0 + 8 * p;
+          if (8 * p % step == 0) {
+            id = -1;
+            if (seen(from, from + step)) {
+              id = row[from >> a.block_log2];
+              if (id < 0 || id >= a.num_blocks) {
+                if (a.error_flag) atomicOr(a.error_flag, 1);
+                id = -1;
+              }
+            }
+          }
+          sid[wave][lane][p] = id;
+        }
+      }
+    }
+    first_tok = t0;
+    bits = __builtin_amdgcn_ballot_w64(keep);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  const int nwords = hi > lo + wave ? (int)(((hi - lo - wave + kPmWaves - 1) / kPmWaves + 63) / 64) : 0;
+  if (nwords) load_word();
+
+  auto sees = [&](int j) { return j < s.L && (s.L - 1 - j < a.window || j < s.prefix); };
+  // the unit at hand: its first token (-1: none), whether every token of it is
+  // seen, the lane's blocks (of its K, and of its V and scores; -1: none)
+  int tok0 = -1, ik = -1, iv = -1;
+  bool full = false;
+  auto next = [&]() {
+    while (bits == 0) {
+      if (++word >= nwords) {
+        tok0 = -1;
+        return;
+      }
+      load_word();
+    }
+    const int i = __builtin_ctzll(bits);
+    bits &= bits - 1;
+    tok0 = __builtin_amdgcn_readlane(first_tok, i);
+    ik = sid[wave][i][x >> 2];
+    iv = sid[wave][i][r];
+    full = tok0 + kPmUnit <= s.L && (s.L - 1 - tok0 < a.window || tok0 + kPmUnit <= s.prefix) &&
+           __builtin_amdgcn_ballot_w64(iv < 0) == 0;
+  };
+  B buf;
+  auto load_k = [&]() {
+    const char* base = a.k + (int64_t)ik * a.k_sb + (int64_t)kv * a.k_sh + 16 * r;
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+      const int j = tok0 + 8 * (x >> 2) + 4 * tb + (x & 3);
+      const char* p = base + (int64_t)(j & (bs - 1)) * a.k_ss;
+      if (full || (ik >= 0 && sees(j))) {
+#pragma unroll
+        for (int w = 0; w < B::KW; w += 4) pm_load<4>(p + 16 * w, buf.k[tb] + w);
+      } else {
+#pragma unroll
+        for (int w = 0; w < B::KW; ++w) buf.k[tb][w] = 0u;
+      }
+    }
+  };
+  auto load_v = [&]() {
+    const char* base = a.v + (int64_t)iv * a.v_sb + (int64_t)kv * a.v_sh + B::CPL * ES * x;
+    const int s0 = (tok0 + 8 * r) & (bs - 1);  // eight slots in a row
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const char* p = base + (int64_t)(s0 + t) * a.v_ss;
+      if (full || (iv >= 0 && sees(tok0 + 8 * r + t))) {
+#pragma unroll
+        for (int c = 0; c < B::CH; ++c) pm_load<B::VW>(p + 16 * B::CPL * ES * c, buf.v[t][c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < B::CH; ++c)
+#pragma unroll
+          for (int w = 0; w < B::VW; ++w) buf.v[t][c][w] = 0u;
+      }
+    }
+  };
+
+  float m = kNoScore, l = 0.f;
+  f32x4 acc[D / 16];
+#pragma unroll
+  for (int nc = 0; nc < D / 16; ++nc) acc[nc] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (nwords) next();
+  if (tok0 >= 0) {
+    load_k();
+    load_v();
+  }
+  while (tok0 >= 0) {
+    f32x4 c[2];
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+      c[tb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dc = 0; dc < D / 32; ++dc) {
+        uint32_t kw[4];
+        if constexpr (F8) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) kw[w] = fp8_pair<MT>(buf.k[tb][2 * dc + w / 2], w & 1);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) kw[w] = buf.k[tb][4 * dc + w];
+        }
+        c[tb] = mfma_qk<MT>(kw, q[dc], c[tb]);
+      }
+    }
+    // the changed scores of tokens tok0 + 8 r + 4 tb + i
+    const float d0 = (float)(s.L - 1 - tok0 - 8 * r);
+    float mt = -__builtin_inff();
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float z = c[tb][i] * ex2;
+        if (capped) z = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), cap2);
+        z = __builtin_fmaf(-slope2, d0 - (float)(4 * tb + i), z);
+        if (!full) z = iv >= 0 && sees(tok0 + 8 * r + 4 * tb + i) ? z : -__builtin_inff();
+        c[tb][i] = z;
+        mt = fmaxf(mt, z);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    next();
+    if (tok0 >= 0) load_k();
+    __builtin_amdgcn_sched_barrier(0);
+    mt = fmaxf(mt, xpair<16>(mt));
+    mt = fmaxf(mt, xpair<32>(mt));
+    // rescaled only once a head's maximum has passed its reference by 8: until
+    // then its probabilities are at most 2^8, of the same relative precision
+    const bool move = mt > m + 8.f;
+    if (__builtin_amdgcn_ballot_w64(move)) {
+      const float mn = move ? mt : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int nc = 0; nc < D / 16; ++nc) acc[nc] *= alpha;
+    }
+    // p as a 16-bit part and the 16-bit rounding of the rest: the matrix cores
+    // have time, and p keeps 16 bits and more
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float p0 = __builtin_amdgcn_exp2f(c[w / 2][2 * (w & 1)] - m);
+      const float p1 = __builtin_amdgcn_exp2f(c[w / 2][2 * (w & 1) + 1] - m);
+      l += p0 + p1;
+      ph[w] = pair16<MT>(p0, p1);
+      const uint32_t hw[1] = {ph[w]};
+      pl[w] = pair16<MT>(p0 - elem<MT>(hw, 0), p1 - elem<MT>(hw, 1));
+    }
+#pragma unroll
+    for (int ch = 0; ch < B::CH; ++ch)
+#pragma unroll
+      for (int cw = 0; cw < B::CPL / 2; ++cw) {  // two columns: word cw of the chunk's 16-bit values
+        uint32_t v[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = F8 ? fp8_pair<MT>(buf.v[t][ch][cw / 2], cw & 1) : buf.v[t][ch][cw % B::VW];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) w[t] = __builtin_amdgcn_perm(v[2 * t + 1], v[2 * t], e ? 0x07060302u : 0x05040100u);
+          f32x4& o = acc[B::CPL * ch + 2 * cw + e];
+          o = mfma_qk<MT>(w, ph, o);
+          o = mfma_qk<MT>(w, pl, o);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    if (tok0 >= 0) load_v();
+  }
+
+  // join the four waves: row 4r + i of acc[nc] is lane 4r + i's column nc
+  l += xpair<16>(l);
+  l += xpair<32>(l);
+  if (r == 0) {
+    sm[wave][x] = m;
+    sl[wave][x] = l;
+  }
+#pragma unroll
+  for (int nc = 0; nc < D / 16; ++nc)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      sacc[wave][x][16 * B::CPL * (nc / B::CPL) + B::CPL * (4 * r + i) + nc % B::CPL] = acc[nc][i];
+  __syncthreads();
+  for (int o = tid; o < ng * D; o += kPmThreads) {
+    const int g = o / D, col = o % D;
+    float M = kNoScore, L = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPmWaves; ++w) M = fmaxf(M, sm[w][g]);
+#pragma unroll
+    for (int w = 0; w < kPmWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][g] - M);
+      L = __builtin_fmaf(sl[w][g], f, L);
+      v = __builtin_fmaf(sacc[w][g][col], f, v);
+    }
+    if (a.P == 1) {
+      store_scalar(a.out + b * a.o_sb + (h0 + g) * a.o_sh + 2 * col, MT, L == 0.f ? 0.f : v * a.v_scale / L);
+    } else {
+      const int64_t rr = ((int64_t)b * a.Hq + h0 + g) * a.P + split;
+      a.pacc[rr * D + col] = v;
+      if (col == 0) {
+        a.pm[rr] = M;
+        a.pl[rr] = L;
+      }
+    }
+  }
+}
+
 // Joins the shares of one (sequence, query head): out = sum w acc / sum w l
 // with w = 2^(m - max m).
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
@@ -271,13 +607,34 @@ int check_paged(const oc_attend_paged_params* p) {
   return check_mods(&p->mods);
 }
 
+// whether the matrix-core kernel takes the call: its shapes, and 16-byte vectors of q, K and V (V rows in lanes of
+// 8 bytes at head_dim 64 and in fp8, which are aligned then too)
+bool paged_tuned(const oc_attend_paged_params* p) {
+  if (p->portable || p->dtype == OC_F32 || p->block_size < 8) return false;
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) return false;
+  const int ces = paged_elem_size(p->cache_dtype);
+  for (int64_t x : {(int64_t)(uintptr_t)p->q, p->q_stride_b * 2, p->q_stride_h * 2, (int64_t)(uintptr_t)p->k,
+                    (int64_t)(uintptr_t)p->v, p->k_stride_b * ces, p->k_stride_h * ces, p->k_stride_s * ces,
+                    p->v_stride_b * ces, p->v_stride_h * ces, p->v_stride_s * ces})
+    if (x % 16) return false;
+  return true;
+}
+
 // Shares of a sequence: about four workgroups per CU, at least four tiles each.
 int paged_splits(const oc_attend_paged_params* p) {
   const int64_t tiles = ((int64_t)p->max_blocks * p->block_size + 63) / 64;
   if (p->num_splits > 0) return (int)std::max<int64_t>(1, std::min<int64_t>(p->num_splits, tiles));
   const int64_t g = p->num_q_heads / p->num_kv_heads;
-  const int64_t blocks = (int64_t)p->num_seqs * p->num_kv_heads * ((g + kPortHeads - 1) / kPortHeads);
+  const int heads = paged_tuned(p) ? kPmHeads : kPortHeads;
+  const int64_t blocks = (int64_t)p->num_seqs * p->num_kv_heads * ((g + heads - 1) / heads);
   return (int)std::max<int64_t>(1, std::min<int64_t>({4 * (int64_t)device_cus() / std::max<int64_t>(blocks, 1), tiles / 4, 1024}));
+}
+
+template <int CT, int MT>
+void launch_paged_mfma(const PagedArgs& a, dim3 grid, hipStream_t s) {
+  if (a.d == 64) hipLaunchKernelGGL((paged_mfma_kernel<CT, MT, 64>), grid, dim3(kPmThreads), 0, s, a);
+  else if (a.d == 128) hipLaunchKernelGGL((paged_mfma_kernel<CT, MT, 128>), grid, dim3(kPmThreads), 0, s, a);
+  else hipLaunchKernelGGL((paged_mfma_kernel<CT, MT, 256>), grid, dim3(kPmThreads), 0, s, a);
 }
 
 }  // namespace
@@ -320,9 +677,16 @@ extern "C" int oc_attend_paged(const oc_attend_paged_params* p, void* stream) {
   const int64_t rows = (int64_t)a.n * a.Hq;
   a.pm = (float*)p->workspace, a.pl = a.pm + rows * a.P, a.pacc = a.pl + rows * a.P;
   const hipStream_t s = (hipStream_t)stream;
-  const int chunks = (a.G + kPortHeads - 1) / kPortHeads;
+  const bool tuned = paged_tuned(p);
+  const int heads = tuned ? kPmHeads : kPortHeads;
+  const int chunks = (a.G + heads - 1) / heads;
   const dim3 grid((unsigned)a.P, (unsigned)(a.Hkv * chunks), (unsigned)a.n);
-  switch (p->cache_dtype) {
+  if (tuned) {
+    if (p->cache_dtype == OC_BF16) launch_paged_mfma<OC_BF16, OC_BF16>(a, grid, s);
+    else if (p->cache_dtype == OC_F16) launch_paged_mfma<OC_F16, OC_F16>(a, grid, s);
+    else if (p->dtype == OC_BF16) launch_paged_mfma<OC_FP8_E4M3FN, OC_BF16>(a, grid, s);
+    else launch_paged_mfma<OC_FP8_E4M3FN, OC_F16>(a, grid, s);
+  } else switch (p->cache_dtype) {
     case OC_F32: hipLaunchKernelGGL(paged_portable_kernel<OC_F32>, grid, dim3(kPortThreads), 0, s, a); break;
     case OC_F16: hipLaunchKernelGGL(paged_portable_kernel<OC_F16>, grid, dim3(kPortThreads), 0, s, a); break;
     case OC_BF16: hipLaunchKernelGGL(paged_portable_kernel<OC_BF16>, grid, dim3(kPortThreads), 0, s, a); break;

@@ -120,6 +120,22 @@ def test_paged(dt, cache, d, g, bs, change, portable):
                      what=f"splits {splits}", **c)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cache", [torch.bfloat16, FP8], ids=str)
+def test_paged_blocks(d, cache):
+    """Blocks of 8 to 1024 tokens (four to a unit of the tuned kernel's, and a unit in a part of one), more query
+    heads to a kv head than one workgroup takes."""
+    import orthocache_gpu as oc
+    for bs, g in ((8, 17), (16, 33), (512, 2), (1024, 16)):
+        lens = [29, 1100, 2500]
+        kc, vc, t = _paged(lens, 1, d, bs, cache, bs, transposed=bs == 8)
+        q = _randn((3, g, d), torch.bfloat16, 1)
+        l32 = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        p32 = torch.tensor([3, 100, 41], dtype=torch.int32, device=DEV)
+        out = oc.attend_paged(q, kc, vc, t, l32, window=901, prefix_lens=p32, alibi_slopes=_slopes(g))
+        _check_paged(out, q, kc, vc, t, lens, window=901, prefix=[3, 100, 41], slopes=_slopes(g), what=f"block {bs}", p_step=_p_step(torch.bfloat16))
+
+
 @pytest.mark.parametrize("d", [8, 24, 80, 96, 192, 512])
 @pytest.mark.parametrize("dt,cache", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, FP8)], ids=str)
 def test_paged_head_dims(d, dt, cache):
