@@ -444,11 +444,12 @@ def _framework():
     if path not in sys.path:
         sys.path.insert(0, path)
     import orthocache_gpu
+    _framework.found = orthocache_gpu
     return orthocache_gpu
 
 
 def _own(s):
-    oc, c = _framework(), s["case"]
+    oc, c = getattr(_framework, "found", None) or _framework(), s["case"]
     kind = c["kind"]
     if kind in ("rotary", "append"):
         table = oc.RotaryTable(s["freq"])
