@@ -32,29 +32,29 @@ from .paged_cache import cache_scales, check_caches, index_tensor, tile_flags
 from .rotary import no_grad_needed
 
 
-def _fill_mods(m: N.OcScoreMods, keep: list, *, scale, softcap, slopes, window, prefix, evict, batch, hq, hkv, d, device):
-    """The score changes in the parameter block; keep holds what it points to."""
-    m.scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(m.scale):
+def _mods(scale, softcap, slopes, window, prefix, evict, batch, hq, hkv, d, device):
+    """The score changes as the library's block, and the tensors it points to."""
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
         raise ValueError(f"scale {scale} must be finite")
     if not (softcap >= 0 and math.isfinite(softcap)):
         raise ValueError(f"softcap {softcap} must be 0 (none) or positive")
     if window < 0:
         raise ValueError(f"window {window} must be 0 (none) or positive")
-    m.softcap, m.window = float(softcap), min(int(window), 2 ** 31 - 1)
+    ptrs = [None, None, None]
+    sb = sh = cols = 0
     if slopes is not None:
-        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (hq,) or slopes.device != device:
+        if slopes.dtype != torch.float32 or slopes.shape != (hq,) or slopes.device != device:
             raise ValueError(f"alibi_slopes must be float32 ({hq},) on {device}")
         slopes = slopes.contiguous()
-        m.slopes = slopes.data_ptr()
+        ptrs[0] = slopes.data_ptr()
     if prefix is not None:
-        prefix = index_tensor(prefix, (batch,), "prefix_lens", device).contiguous()
-        m.prefix_lens = prefix.data_ptr()
+        prefix = index_tensor(prefix, (batch,), "prefix_lens", device)
+        ptrs[1] = prefix.data_ptr()
     if evict is not None:
         evict = tile_flags(evict, batch, hkv, device)
-        m.evict, m.evict_stride_b, m.evict_stride_h = evict.data_ptr(), evict.stride(0), evict.stride(1)
-        m.evict_cols = evict.shape[2]
-    keep += [slopes, prefix, evict]
+        ptrs[2], (sb, sh), cols = evict.data_ptr(), evict.stride()[:2], evict.shape[2]
+    return (N.OcScoreMods(scale, softcap, *ptrs, sb, sh, cols, min(int(window), 2 ** 31 - 1)), (slopes, prefix, evict))
 
 
 def attend_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -93,38 +93,28 @@ def attend_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
         raise TypeError(f"the cache must have q's dtype ({q.dtype}) or float8_e4m3fn, got {k_cache.dtype}")
     cache_scales(k_cache.dtype, k_scale, v_scale)
     block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
-    context_lens = index_tensor(context_lens, (n,), "context_lens", device).contiguous()
+    context_lens = index_tensor(context_lens, (n,), "context_lens", device)
     if num_splits is not None and num_splits < 1:
         raise ValueError(f"num_splits ({num_splits}) must be positive")
     if out is None:
         out = torch.empty((n, hq, d), dtype=q.dtype, device=device)
-    elif tuple(out.shape) != (n, hq, d) or out.dtype != q.dtype or out.device != device or (d > 1 and out.stride(2) != 1):
+    elif out.shape != (n, hq, d) or out.dtype != q.dtype or out.device != device or (d > 1 and out.stride(2) != 1):
         raise ValueError(f"out must be a ({n}, {hq}, {d}) {q.dtype} tensor on {device} with a contiguous last dim")
     q = X.ready16(q)
-    p = N.OcAttendPagedParams()
-    keep = []
-    _fill_mods(p.mods, keep, scale=scale, softcap=softcap, slopes=alibi_slopes, window=window, prefix=prefix_lens,
-               evict=evict_mask, batch=n, hq=hq, hkv=hkv, d=d, device=device)
-    p.q, p.q_stride_b, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    p.k, p.v = k_cache.data_ptr(), v_cache.data_ptr()
-    p.k_stride_b, p.k_stride_h, p.k_stride_s = k_cache.stride()[:3]
-    p.v_stride_b, p.v_stride_h, p.v_stride_s = v_cache.stride()[:3]
-    p.block_tables, p.bt_stride, p.num_blocks = block_tables.data_ptr(), block_tables.stride(0), nb
-    p.context_lens, p.max_blocks, p.block_size = context_lens.data_ptr(), block_tables.shape[1], bs
-    p.dtype, p.cache_dtype = dt, X.dtype_code(k_cache.dtype, "cache")
-    p.num_seqs, p.num_q_heads, p.num_kv_heads, p.head_dim = n, hq, hkv, d
-    p.k_scale, p.v_scale, p.num_splits, p.portable = k_scale, v_scale, num_splits or 0, bool(portable)
-    p.out, p.out_stride_b, p.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    mods, held = _mods(scale, softcap, alibi_slopes, window, prefix_lens, evict_mask, n, hq, hkv, d, device)
     flag = torch.zeros(1, dtype=torch.int32, device=device) if sync else None
-    p.error_flag = X._ptr(flag)
-    lib = N.lib()
-    with torch.cuda.device(device):
-        need = lib.oc_attend_paged_workspace_size(ctypes.byref(p))
-        if need:
-            # a buffer of the call's own: two captured graphs replayed at once share nothing
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        N.check("oc_attend_paged", lib.oc_attend_paged(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    qs, ks, vs, os = q.stride(), k_cache.stride(), v_cache.stride(), out.stride()
+    p = N.OcAttendPagedParams(
+        q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        block_tables.data_ptr(), block_tables.stride(0), nb, context_lens.data_ptr(), block_tables.shape[1], bs, dt,
+        X.dtype_code(k_cache.dtype, "cache"), n, hq, hkv, d, k_scale, v_scale, mods, num_splits or 0, bool(portable),
+        out.data_ptr(), os[0], os[1], X._ptr(flag))
+    need = N.lib().oc_attend_paged_workspace_size(ctypes.byref(p))
+    if need:
+        # a buffer of the call's own: two captured graphs replayed at once share nothing
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    X.launch("oc_attend_paged", p, device)
     if flag is not None and int(flag.item()):
         raise ValueError("block_tables holds a block id outside [0, num_blocks)")
     return out
@@ -151,27 +141,21 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: O
     dt = X.dtype_code(q.dtype, "q", allow_fp8=False)
     if d not in (64, 128):
         raise NotImplementedError(f"head_dim {d} is not supported (64 or 128)")
-    p = N.OcAttendPromptParams()
-    keep = []
-    _fill_mods(p.mods, keep, scale=scale, softcap=softcap, slopes=alibi_slopes, window=window, prefix=prefix_lens,
-               evict=evict_mask, batch=B, hq=hq, hkv=hkv, d=d, device=device)
+    mods, held = _mods(scale, softcap, alibi_slopes, window, prefix_lens, evict_mask, B, hq, hkv, d, device)
+    docs, docs_sb = None, 0
     if documents is not None:
         if documents.dim() == 1:
             documents = documents.unsqueeze(0).expand(B, -1)
         documents = index_tensor(documents, (B, skv), "documents", device)
-        p.documents, p.documents_stride_b = documents.data_ptr(), documents.stride(0)
+        docs, docs_sb = documents.data_ptr(), documents.stride(0)
     q, k, v = X.ready16(q), X.ready16(k, 2), X.ready16(v, 2)
     out = torch.empty((B, hq, sq, d), dtype=q.dtype, device=device)
-    p.q, (p.q_stride_b, p.q_stride_h, p.q_stride_s) = q.data_ptr(), q.stride()[:3]
-    p.k, (p.k_stride_b, p.k_stride_h, p.k_stride_s) = k.data_ptr(), k.stride()[:3]
-    p.v, (p.v_stride_b, p.v_stride_h, p.v_stride_s) = v.data_ptr(), v.stride()[:3]
-    p.out, (p.out_stride_b, p.out_stride_h, p.out_stride_s) = out.data_ptr(), out.stride()[:3]
-    p.dtype, p.batch, p.num_q_heads, p.num_kv_heads, p.q_len, p.kv_len, p.head_dim = dt, B, hq, hkv, sq, skv, d
-    lib = N.lib()
-    with torch.cuda.device(device):
-        need = lib.oc_attend_prompt_workspace_size(ctypes.byref(p))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        N.check("oc_attend_prompt", lib.oc_attend_prompt(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    p = N.OcAttendPromptParams(
+        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], out.data_ptr(),
+        *out.stride()[:3], dt, B, hq, hkv, sq, skv, d, docs, docs_sb, mods)
+    if docs is not None:
+        need = N.lib().oc_attend_prompt_workspace_size(ctypes.byref(p))
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    X.launch("oc_attend_prompt", p, device)
     return out

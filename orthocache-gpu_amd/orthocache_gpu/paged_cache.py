@@ -31,14 +31,16 @@ def index_tensor(t: torch.Tensor, shape: Tuple[int, ...], what: str, device: tor
         raise TypeError(f"{what} must be int32, got {t.dtype}")
     if t.device != device:
         raise RuntimeError(f"orthocache_gpu: {what} on {t.device}, the rest on {device}")
-    if t.dim() != len(shape) or any(n not in (-1, m) for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{what} must be {shape}, got {tuple(t.shape)}")
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    got = t.shape
+    if got != shape:
+        if len(got) != len(shape) or any(n not in (-1, m) for n, m in zip(shape, got)):
+            raise ValueError(f"{what} must be {shape}, got {tuple(got)}")
+    return t if t.is_contiguous() or got[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: Tuple[int, ...]) -> None:
     if k_cache.dim() not in dims or v_cache.shape != k_cache.shape:
-        raise ValueError(f"k_cache and v_cache must be {' or '.join(str(d) + '-D' for d in dims)} of one shape, got "
+        raise ValueError(f"k_cache and v_cache must be {' or '.join(str(n) + '-D' for n in dims)} of one shape, got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     if k_cache.dtype != v_cache.dtype:
         raise TypeError(f"k_cache and v_cache must share a dtype ({k_cache.dtype}, {v_cache.dtype})")
@@ -46,13 +48,12 @@ def check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: Tuple[int, 
     bs = k_cache.shape[-2]
     if bs < 1 or bs & (bs - 1):
         raise ValueError(f"block_size ({bs}) must be a power of 2")
-    for t in (k_cache, v_cache):
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError("cache rows must be contiguous along head_dim")
+    if k_cache.shape[-1] > 1 and (k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1):
+        raise ValueError("cache rows must be contiguous along head_dim")
 
 
-def written_caches(*caches: torch.Tensor) -> None:
-    if any(overlaps(t) for t in caches):
+def written_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    if overlaps(k_cache) or overlaps(v_cache):
         raise ValueError("elements of a cache that is written may not share memory")
 
 
@@ -96,7 +97,7 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     written_caches(k_cache, v_cache)
     nb, hkv, bs, d = k_cache.shape
     tokens = k.shape[0]
-    if tuple(k.shape) != (tokens, hkv, d) or v.shape != k.shape:
+    if k.shape != (tokens, hkv, d) or v.shape != k.shape:
         raise ValueError(f"k and v must be (tokens, {hkv}, {d}), got {tuple(k.shape)} and {tuple(v.shape)}")
     if q is not None and (q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != d):
         raise ValueError(f"q must be ({tokens}, heads, {d}), got {tuple(q.shape)}")
@@ -105,50 +106,41 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     cache_scales(k_cache.dtype, k_scale, v_scale)
     n = context_lens.shape[0] if context_lens.dim() == 1 else -1
     context_lens = index_tensor(context_lens, (n,), "context_lens", device)
-    if not context_lens.is_contiguous():
-        context_lens = context_lens.contiguous()
     block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
     if cu_seqlens is not None:
         cu_seqlens = index_tensor(cu_seqlens, (n + 1,), "cu_seqlens", device)
     elif tokens != n:
         raise ValueError(f"{tokens} tokens for {n} sequences need cu_seqlens")
     rot = check_table(table, d, layout, device)
-    p = N.OcAppendParams()
-    p.dtype = X.dtype_code(k.dtype, "k", allow_fp8=False)
-    p.cache_dtype = X.dtype_code(k_cache.dtype, "cache")
+    dt = X.dtype_code(k.dtype, "k", allow_fp8=False)
     if positions is not None:
-        if tuple(positions.shape) != (tokens,):
+        if positions.shape != (tokens,):
             raise ValueError(f"positions must be ({tokens},), got {tuple(positions.shape)}")
         positions = check_positions(positions, device)
-        p.positions, p.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
-    k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
-    p.k, p.k_stride_s, p.k_stride_h = k.data_ptr(), k.stride(0), k.stride(1)
-    p.v, p.v_stride_s, p.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
-    out = None
+    if k.stride(-1) != 1:
+        k = k.contiguous()
+    if v.stride(-1) != 1:
+        v = v.contiguous()
+    out, qp, op, hq = None, None, None, 0
+    qs = os = (0, 0)
     if q is not None:
         if q.stride(-1) != 1:
             q = q.contiguous()
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        p.q, p.q_stride_s, p.q_stride_h, p.num_q_heads = q.data_ptr(), q.stride(0), q.stride(1), q.shape[1]
-        p.q_out, p.q_out_stride_s, p.q_out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
         if n == 0:
             out.zero_()
-    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    p.k_cache_stride_b, p.k_cache_stride_h, p.k_cache_stride_s = k_cache.stride()[:3]
-    p.v_cache_stride_b, p.v_cache_stride_h, p.v_cache_stride_s = v_cache.stride()[:3]
-    p.tokens, p.num_seqs, p.num_kv_heads, p.head_dim, p.rotary_dim = tokens, n, hkv, d, rot
-    p.block_size, p.max_blocks, p.num_blocks = bs, block_tables.shape[1], nb
-    p.block_tables, p.bt_stride = block_tables.data_ptr(), block_tables.stride(0)
-    p.context_lens = context_lens.data_ptr()
-    p.cu_seqlens = None if cu_seqlens is None else cu_seqlens.data_ptr()
-    p.interleaved = layout == "interleaved"
-    if table is not None:
-        p.inv_freq, p.scale = table.inv_freq.data_ptr(), table.scale
-    p.k_scale, p.v_scale = k_scale, v_scale
+        qp, op, hq, qs, os = q.data_ptr(), out.data_ptr(), q.shape[1], q.stride(), out.stride()
+    ks, vs, kcs, vcs = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
     flag = torch.zeros(1, dtype=torch.int32, device=device) if sync else None
-    p.error_flag = None if flag is None else flag.data_ptr()
-    with torch.cuda.device(device):
-        N.check("oc_append_paged", N.lib().oc_append_paged(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    p = N.OcAppendParams(
+        qp, k.data_ptr(), v.data_ptr(), op, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+        k_cache.data_ptr(), v_cache.data_ptr(), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2],
+        dt, X.dtype_code(k_cache.dtype, "cache"), tokens, n, hq, hkv, d, rot, bs, block_tables.shape[1], nb,
+        block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), X._ptr(cu_seqlens), X._ptr(positions),
+        positions is not None and positions.dtype == torch.int64, layout == "interleaved",
+        None if table is None else table.inv_freq.data_ptr(), 1.0 if table is None else table.scale, k_scale, v_scale,
+        X._ptr(flag))
+    X.launch("oc_append_paged", p, device)
     if flag is not None and int(flag.item()):
         raise ValueError("block_tables holds no block in [0, num_blocks) for some of the tokens")
     return out
@@ -181,8 +173,10 @@ class PageTables:
 
 def _out_tables(out: Optional[PageTables], rows: int, cols: int, blocks: int, device: torch.device, *inputs) -> PageTables:
     if out is None:
-        new = [torch.empty(s, dtype=torch.int32, device=device) for s in ((rows, cols), (rows,), (blocks,), (1,))]
-        return PageTables(*new)
+        # one allocation: the tables, the lengths, the counts and the status
+        flat = torch.empty(rows * cols + rows + blocks + 1, dtype=torch.int32, device=device)
+        t, l, r, s = flat.split((rows * cols, rows, blocks, 1))
+        return PageTables(t.view(rows, cols), l, r, s)
     for t, shape, what in ((out.block_tables, (rows, cols), "block_tables"), (out.context_lens, (rows,), "context_lens"),
                            (out.ref_counts, (blocks,), "ref_counts"), (out.status, (1,), "status")):
         if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
@@ -246,30 +240,21 @@ def fork_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
         if new_tokens < 0:
             raise ValueError(f"new_tokens {new_tokens} is negative")
         new_tokens = None if new_tokens == 0 else torch.full((children,), int(new_tokens), dtype=torch.int32, device=device)
-    context_lens, ref_counts, parents, new_tokens = (
-        None if t is None else t.contiguous() for t in (context_lens, ref_counts, parents, new_tokens))
     cols = block_tables.shape[1] if max_blocks is None else int(max_blocks)
     if cols < 0:
         raise ValueError(f"max_blocks {cols} is negative")
     res = _out_tables(out, children, cols, nb, device, block_tables, context_lens, ref_counts, parents, new_tokens)
-    p = N.OcForkParams()
-    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    p.k_stride_l, p.k_stride_b, p.k_stride_h, p.k_stride_s = k_cache.stride()[:4]
-    p.v_stride_l, p.v_stride_b, p.v_stride_h, p.v_stride_s = v_cache.stride()[:4]
-    p.cache_dtype = X.dtype_code(k_cache.dtype, "cache")
-    p.layers, p.num_kv_heads, p.head_dim, p.block_size = (layers if nb else 0), hkv, d, bs
-    p.num_seqs, p.num_children, p.max_blocks, p.out_max_blocks, p.num_blocks = n, children, block_tables.shape[1], cols, nb
-    p.block_tables, p.bt_stride = block_tables.data_ptr(), block_tables.stride(0)
-    p.context_lens, p.ref_counts = context_lens.data_ptr(), ref_counts.data_ptr()
-    p.parents, p.new_tokens = X._ptr(parents), X._ptr(new_tokens)
-    p.out_block_tables, p.out_bt_stride = res.block_tables.data_ptr(), res.block_tables.stride(0)
-    p.out_context_lens, p.out_ref_counts = res.context_lens.data_ptr(), res.ref_counts.data_ptr()
-    p.status = res.status.data_ptr()
-    lib = N.lib()
-    ws = torch.empty(max(lib.oc_fork_pages_workspace_size(ctypes.byref(p)), 1), dtype=torch.uint8, device=device)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-    with torch.cuda.device(device):
-        N.check("oc_fork_pages", lib.oc_fork_pages(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    ks, vs = k_cache.stride(), v_cache.stride()
+    p = N.OcForkParams(
+        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3],
+        X.dtype_code(k_cache.dtype, "cache"), layers if nb else 0, hkv, d, bs, n, children, block_tables.shape[1], cols, nb,
+        block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), ref_counts.data_ptr(), X._ptr(parents),
+        X._ptr(new_tokens), res.block_tables.data_ptr(), res.block_tables.stride(0), res.context_lens.data_ptr(),
+        res.ref_counts.data_ptr(), res.status.data_ptr())
+    need = N.lib().oc_fork_pages_workspace_size(ctypes.byref(p))
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    X.launch("oc_fork_pages", p, device)
     return res.check() if sync else res
 
 
@@ -293,9 +278,9 @@ def evict_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_coun
     tokens.  With sync, a block id outside the cache raises ValueError."""
     device = X.require_gpu(block_tables, context_lens, ref_counts, evict_mask)
     n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    context_lens = index_tensor(context_lens, (n,), "context_lens", device).contiguous()
+    context_lens = index_tensor(context_lens, (n,), "context_lens", device)
     block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
-    ref_counts = index_tensor(ref_counts, (-1,), "ref_counts", device).contiguous()
+    ref_counts = index_tensor(ref_counts, (-1,), "ref_counts", device)
     if block_size < 1 or X.TILE_SIZE % block_size:
         raise ValueError(f"block_size ({block_size}) must divide a tile of {X.TILE_SIZE} tokens")
     evict_mask = tile_flags(evict_mask.unsqueeze(1) if evict_mask.dim() == 2 else evict_mask, n, -1, device)
@@ -303,17 +288,12 @@ def evict_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_coun
     tiles = -(-cols * block_size // X.TILE_SIZE)
     res = _out_tables(out, n, cols, nb, device, block_tables, context_lens, ref_counts, evict_mask)
     tile_map = torch.empty((n, tiles), dtype=torch.int32, device=device)
-    p = N.OcEvictParams()
-    p.num_seqs, p.num_kv_heads, p.block_size, p.max_blocks, p.num_blocks = n, evict_mask.shape[1], block_size, cols, nb
-    p.block_tables, p.bt_stride = block_tables.data_ptr(), block_tables.stride(0)
-    p.context_lens, p.ref_counts = context_lens.data_ptr(), ref_counts.data_ptr()
-    p.evict, p.evict_stride_b, p.evict_stride_h = evict_mask.data_ptr(), evict_mask.stride(0), evict_mask.stride(1)
-    p.evict_cols, p.tile_map_cols = evict_mask.shape[2], tiles
-    p.out_block_tables, p.out_bt_stride = res.block_tables.data_ptr(), res.block_tables.stride(0)
-    p.out_context_lens, p.out_ref_counts = res.context_lens.data_ptr(), res.ref_counts.data_ptr()
-    p.tile_map, p.status = tile_map.data_ptr(), res.status.data_ptr()
-    with torch.cuda.device(device):
-        N.check("oc_evict_pages", N.lib().oc_evict_pages(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    p = N.OcEvictParams(
+        n, evict_mask.shape[1], block_size, cols, nb, block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
+        ref_counts.data_ptr(), evict_mask.data_ptr(), evict_mask.stride(0), evict_mask.stride(1), evict_mask.shape[2], tiles,
+        res.block_tables.data_ptr(), res.block_tables.stride(0), res.context_lens.data_ptr(), res.ref_counts.data_ptr(),
+        tile_map.data_ptr(), res.status.data_ptr())
+    X.launch("oc_evict_pages", p, device)
     return (res.check() if sync else res), tile_map
 
 

@@ -8,7 +8,6 @@ themselves, on tensors here and on the way into a paged cache in
 
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 from typing import Dict, Optional
@@ -98,12 +97,15 @@ def check_positions(positions: torch.Tensor, device: torch.device) -> torch.Tens
 def no_grad_needed(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """These operators record no gradient: an input that wants one is refused
     rather than cut off silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad(), or detach its inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} records no gradient: call it under torch.no_grad(), or detach its inputs")
 
 
 def overlaps(t: torch.Tensor) -> bool:
     """Whether elements of t may share memory (an expanded view, say)."""
+    if t.is_contiguous():
+        return False
     reach = 0  # of the elements along the dimensions of smaller strides
     for st, n in sorted((abs(s), n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if st <= reach:
@@ -145,9 +147,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if tuple(positions.shape) not in ((tokens,), (batch, tokens)):
         raise ValueError(f"positions must be ({tokens},) or ({batch}, {tokens}), got {tuple(positions.shape)}")
     positions = check_positions(positions, device)
-    p = N.OcRotaryParams()
-    ys = []
-    for i, x in enumerate(xs):
+    ys, ptrs, heads = [], [], []
+    for x in xs:
         if inplace:
             if (x.stride(-1) != 1 and d > 1) or overlaps(x):
                 raise ValueError("in place, the last dimension must be contiguous and no elements may share memory")
@@ -159,21 +160,19 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
             if y.stride(-1) != 1:
                 y = torch.empty(x.shape, dtype=x.dtype, device=device)
         ys.append(y)
-        for t, name in ((x, "x"), (y, "y")):
-            st = t.stride()
-            b, h, s = (0, st[1], st[0]) if t.dim() == 3 else st[:3]
-            getattr(p, name)[i] = t.data_ptr()
-            getattr(p, name + "_stride_b")[i] = b
-            getattr(p, name + "_stride_h")[i] = h
-            getattr(p, name + "_stride_s")[i] = s
-        p.heads[i] = x.shape[1]
-    if inplace and k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
+        xst, yst = x.stride(), y.stride()
+        if len(xst) == 3:  # (tokens, heads, d)
+            xst, yst = (0, xst[1], xst[0]), (0, yst[1], yst[0])
+        ptrs.append((x.data_ptr(), y.data_ptr(), *xst[:3], *yst[:3]))
+        heads.append(x.shape[1])
+    if k is None:
+        ptrs.append((None, None, 0, 0, 0, 0, 0, 0))
+        heads.append(0)
+    elif inplace and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
         raise ValueError("in place, q and k must be different tensors")
-    p.dtype, p.batch, p.tokens, p.head_dim, p.rotary_dim = dt, batch, tokens, d, rot
-    p.interleaved, p.backward = layout == "interleaved", backward
-    p.positions, p.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
-    p.positions_stride_b = positions.stride(0) if positions.dim() == 2 and batch > 1 else 0
-    p.inv_freq, p.scale = table.inv_freq.data_ptr(), table.scale
-    with torch.cuda.device(device):
-        N.check("oc_apply_rotary", N.lib().oc_apply_rotary(ctypes.byref(p), ctypes.c_void_p(X.current_stream(device))))
+    p = N.OcRotaryParams(
+        *zip(*ptrs), tuple(heads), dt, batch, tokens, d, rot, layout == "interleaved", backward,
+        positions.dtype == torch.int64, positions.data_ptr(),
+        positions.stride(0) if positions.dim() == 2 and batch > 1 else 0, table.inv_freq.data_ptr(), table.scale)
+    X.launch("oc_apply_rotary", p, device)
     return ys[0] if k is None else tuple(ys)
