@@ -285,19 +285,6 @@ def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch(name: str, p: ctypes.Structure, device: torch.device) -> None:
-    """name(&p, the current stream of device) with device the current one (the
-    device guard costs 2 us, so it is taken only where it changes something)."""
-    fn = getattr(N.lib(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(p), current_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.byref(p), current_stream(device))
-    if rc:
-        N.check(name, rc)
-
-
 # ---------------------------------------------------------------- split count
 
 _CU_COUNT: Dict[int, int] = {}

@@ -8,63 +8,17 @@ reference fills it by hand and has no operator that changes a block table.
 
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
 
-from . import _launch as X
 from . import _native as N
-from .rotary import RotaryTable, check_positions, check_table, no_grad_needed, overlaps
-
-MAX_SEQS = 4096  # sequences and children of a fork
-
+from ._ops import number, ops
+from .rotary import RotaryTable
 
 class OutOfPages(RuntimeError):
     """A call needs more free blocks than the cache has."""
-
-
-def index_tensor(t: torch.Tensor, shape: Tuple[int, ...], what: str, device: torch.device) -> torch.Tensor:
-    """An int32 tensor of the shape (-1: any size) with a contiguous last dimension."""
-    if t.dtype != torch.int32:
-        raise TypeError(f"{what} must be int32, got {t.dtype}")
-    if t.device != device:
-        raise RuntimeError(f"orthocache_gpu: {what} on {t.device}, the rest on {device}")
-    got = t.shape
-    if got != shape:
-        if len(got) != len(shape) or any(n not in (-1, m) for n, m in zip(shape, got)):
-            raise ValueError(f"{what} must be {shape}, got {tuple(got)}")
-    return t if t.is_contiguous() or got[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: Tuple[int, ...]) -> None:
-    if k_cache.dim() not in dims or v_cache.shape != k_cache.shape:
-        raise ValueError(f"k_cache and v_cache must be {' or '.join(str(n) + '-D' for n in dims)} of one shape, got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if k_cache.dtype != v_cache.dtype:
-        raise TypeError(f"k_cache and v_cache must share a dtype ({k_cache.dtype}, {v_cache.dtype})")
-    X.dtype_code(k_cache.dtype, "cache")
-    bs = k_cache.shape[-2]
-    if bs < 1 or bs & (bs - 1):
-        raise ValueError(f"block_size ({bs}) must be a power of 2")
-    if k_cache.shape[-1] > 1 and (k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1):
-        raise ValueError("cache rows must be contiguous along head_dim")
-
-
-def written_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    if overlaps(k_cache) or overlaps(v_cache):
-        raise ValueError("elements of a cache that is written may not share memory")
-
-
-def cache_scales(dtype: torch.dtype, *scales: float) -> None:
-    for s in scales:
-        if isinstance(s, torch.Tensor):
-            raise TypeError("k_scale and v_scale are numbers here")
-        if not (s > 0 and s < float("inf")):
-            raise ValueError(f"scales must be positive and finite, got {s}")
-        if s != 1.0 and dtype != torch.float8_e4m3fn:
-            raise ValueError(f"k_scale and v_scale are for float8_e4m3fn caches, not {dtype}")
 
 
 def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -91,59 +45,9 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     (`fork_pages` sees to that).  With sync, a block id outside [0, num_blocks)
     and a table too short for a token raise ValueError; without, such tokens
     are left out."""
-    no_grad_needed("append_paged", q, k, v)
-    device = X.require_gpu(k, v, k_cache, v_cache, block_tables, context_lens, q)
-    check_caches(k_cache, v_cache, (4,))
-    written_caches(k_cache, v_cache)
-    nb, hkv, bs, d = k_cache.shape
-    tokens = k.shape[0]
-    if k.shape != (tokens, hkv, d) or v.shape != k.shape:
-        raise ValueError(f"k and v must be (tokens, {hkv}, {d}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    if q is not None and (q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != d):
-        raise ValueError(f"q must be ({tokens}, heads, {d}), got {tuple(q.shape)}")
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
-        raise TypeError("q, k and v must share a dtype")
-    cache_scales(k_cache.dtype, k_scale, v_scale)
-    n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    context_lens = index_tensor(context_lens, (n,), "context_lens", device)
-    block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
-    if cu_seqlens is not None:
-        cu_seqlens = index_tensor(cu_seqlens, (n + 1,), "cu_seqlens", device)
-    elif tokens != n:
-        raise ValueError(f"{tokens} tokens for {n} sequences need cu_seqlens")
-    rot = check_table(table, d, layout, device)
-    dt = X.dtype_code(k.dtype, "k", allow_fp8=False)
-    if positions is not None:
-        if positions.shape != (tokens,):
-            raise ValueError(f"positions must be ({tokens},), got {tuple(positions.shape)}")
-        positions = check_positions(positions, device)
-    if k.stride(-1) != 1:
-        k = k.contiguous()
-    if v.stride(-1) != 1:
-        v = v.contiguous()
-    out, qp, op, hq = None, None, None, 0
-    qs = os = (0, 0)
-    if q is not None:
-        if q.stride(-1) != 1:
-            q = q.contiguous()
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        if n == 0:
-            out.zero_()
-        qp, op, hq, qs, os = q.data_ptr(), out.data_ptr(), q.shape[1], q.stride(), out.stride()
-    ks, vs, kcs, vcs = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
-    flag = torch.zeros(1, dtype=torch.int32, device=device) if sync else None
-    p = N.OcAppendParams(
-        qp, k.data_ptr(), v.data_ptr(), op, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
-        k_cache.data_ptr(), v_cache.data_ptr(), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2],
-        dt, X.dtype_code(k_cache.dtype, "cache"), tokens, n, hq, hkv, d, rot, bs, block_tables.shape[1], nb,
-        block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), X._ptr(cu_seqlens), X._ptr(positions),
-        positions is not None and positions.dtype == torch.int64, layout == "interleaved",
-        None if table is None else table.inv_freq.data_ptr(), 1.0 if table is None else table.scale, k_scale, v_scale,
-        X._ptr(flag))
-    X.launch("oc_append_paged", p, device)
-    if flag is not None and int(flag.item()):
-        raise ValueError("block_tables holds no block in [0, num_blocks) for some of the tokens")
-    return out
+    freq, scale = (None, 1.0) if table is None else (table.inv_freq, table.scale)
+    return ops().append_paged(k, v, k_cache, v_cache, block_tables, context_lens, q, cu_seqlens, positions, freq, scale,
+                              layout, number(k_scale, "k_scale"), number(v_scale, "v_scale"), sync)
 
 
 @dataclass
@@ -171,23 +75,8 @@ class PageTables:
         return self
 
 
-def _out_tables(out: Optional[PageTables], rows: int, cols: int, blocks: int, device: torch.device, *inputs) -> PageTables:
-    if out is None:
-        # one allocation: the tables, the lengths, the counts and the status
-        flat = torch.empty(rows * cols + rows + blocks + 1, dtype=torch.int32, device=device)
-        t, l, r, s = flat.split((rows * cols, rows, blocks, 1))
-        return PageTables(t.view(rows, cols), l, r, s)
-    for t, shape, what in ((out.block_tables, (rows, cols), "block_tables"), (out.context_lens, (rows,), "context_lens"),
-                           (out.ref_counts, (blocks,), "ref_counts"), (out.status, (1,), "status")):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-            raise ValueError(f"out.{what} must be a contiguous int32 {shape} tensor on {device}")
-        lo, hi = t.data_ptr(), t.data_ptr() + 4 * t.numel()
-        for i in inputs:
-            if i is not None and i.numel() and t.numel():
-                reach = i.element_size() * (1 + sum((m - 1) * s for m, s in zip(i.shape, i.stride())))
-                if i.data_ptr() < hi and lo < i.data_ptr() + reach:
-                    raise ValueError(f"out.{what} overlaps an input: the old tables must stay")
-    return out
+def _parts(out: Optional[PageTables]):
+    return None if out is None else (out.block_tables, out.context_lens, out.ref_counts, out.status)
 
 
 def fork_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -218,43 +107,9 @@ def fork_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
     sequence's number, a block id outside the cache or a table too narrow;
     without, the result's status says so.  Then nothing is copied and the new
     tables are empty."""
-    device = X.require_gpu(k_cache, v_cache, block_tables, context_lens, ref_counts, parents)
-    check_caches(k_cache, v_cache, (4, 5))
-    written_caches(k_cache, v_cache)
-    if k_cache.dim() == 4:
-        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    layers, nb, hkv, bs, d = k_cache.shape
-    n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    context_lens = index_tensor(context_lens, (n,), "context_lens", device)
-    block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
-    ref_counts = index_tensor(ref_counts, (nb,), "ref_counts", device)
-    children = n
-    if parents is not None:
-        parents = index_tensor(parents, (-1,), "parents", device)
-        children = parents.shape[0]
-    if max(n, children) > MAX_SEQS:
-        raise NotImplementedError(f"at most {MAX_SEQS} sequences and children, got {n} and {children}")
-    if isinstance(new_tokens, torch.Tensor):
-        new_tokens = index_tensor(new_tokens, (children,), "new_tokens", device)
-    else:
-        if new_tokens < 0:
-            raise ValueError(f"new_tokens {new_tokens} is negative")
-        new_tokens = None if new_tokens == 0 else torch.full((children,), int(new_tokens), dtype=torch.int32, device=device)
-    cols = block_tables.shape[1] if max_blocks is None else int(max_blocks)
-    if cols < 0:
-        raise ValueError(f"max_blocks {cols} is negative")
-    res = _out_tables(out, children, cols, nb, device, block_tables, context_lens, ref_counts, parents, new_tokens)
-    ks, vs = k_cache.stride(), v_cache.stride()
-    p = N.OcForkParams(
-        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3],
-        X.dtype_code(k_cache.dtype, "cache"), layers if nb else 0, hkv, d, bs, n, children, block_tables.shape[1], cols, nb,
-        block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(), ref_counts.data_ptr(), X._ptr(parents),
-        X._ptr(new_tokens), res.block_tables.data_ptr(), res.block_tables.stride(0), res.context_lens.data_ptr(),
-        res.ref_counts.data_ptr(), res.status.data_ptr())
-    need = N.lib().oc_fork_pages_workspace_size(ctypes.byref(p))
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), need
-    X.launch("oc_fork_pages", p, device)
+    each, every = (new_tokens, 0) if isinstance(new_tokens, torch.Tensor) else (None, new_tokens)
+    res = PageTables(*ops().fork_pages(k_cache, v_cache, block_tables, context_lens, ref_counts, parents, each, every,
+                                       max_blocks, _parts(out)))
     return res.check() if sync else res
 
 
@@ -276,33 +131,6 @@ def evict_pages(block_tables: torch.Tensor, context_lens: torch.Tensor, ref_coun
     positions then: append_paged takes the positions of the next tokens, while
     the window, the prefix and the distance of attend_paged count cached
     tokens.  With sync, a block id outside the cache raises ValueError."""
-    device = X.require_gpu(block_tables, context_lens, ref_counts, evict_mask)
-    n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    context_lens = index_tensor(context_lens, (n,), "context_lens", device)
-    block_tables = index_tensor(block_tables, (n, -1), "block_tables", device)
-    ref_counts = index_tensor(ref_counts, (-1,), "ref_counts", device)
-    if block_size < 1 or X.TILE_SIZE % block_size:
-        raise ValueError(f"block_size ({block_size}) must divide a tile of {X.TILE_SIZE} tokens")
-    evict_mask = tile_flags(evict_mask.unsqueeze(1) if evict_mask.dim() == 2 else evict_mask, n, -1, device)
-    cols, nb = block_tables.shape[1], ref_counts.shape[0]
-    tiles = -(-cols * block_size // X.TILE_SIZE)
-    res = _out_tables(out, n, cols, nb, device, block_tables, context_lens, ref_counts, evict_mask)
-    tile_map = torch.empty((n, tiles), dtype=torch.int32, device=device)
-    p = N.OcEvictParams(
-        n, evict_mask.shape[1], block_size, cols, nb, block_tables.data_ptr(), block_tables.stride(0), context_lens.data_ptr(),
-        ref_counts.data_ptr(), evict_mask.data_ptr(), evict_mask.stride(0), evict_mask.stride(1), evict_mask.shape[2], tiles,
-        res.block_tables.data_ptr(), res.block_tables.stride(0), res.context_lens.data_ptr(), res.ref_counts.data_ptr(),
-        tile_map.data_ptr(), res.status.data_ptr())
-    X.launch("oc_evict_pages", p, device)
+    *tables, tile_map = ops().evict_pages(block_tables, context_lens, ref_counts, evict_mask, block_size, _parts(out))
+    res = PageTables(*tables)
     return (res.check() if sync else res), tile_map
-
-
-def tile_flags(mask: torch.Tensor, batch: int, heads: int, device: torch.device) -> torch.Tensor:
-    """A (batch, heads, tiles) bool or uint8 mask with a contiguous last dimension (heads -1: any, at least one)."""
-    if mask.dtype not in (torch.bool, torch.uint8):
-        raise TypeError(f"evict_mask must be bool or uint8, got {mask.dtype}")
-    if mask.device != device:
-        raise RuntimeError(f"orthocache_gpu: evict_mask on {mask.device}, the rest on {device}")
-    if mask.dim() != 3 or mask.shape[0] != batch or (mask.shape[1] != heads if heads >= 0 else mask.shape[1] < 1):
-        raise ValueError(f"evict_mask must be ({batch}, {heads if heads >= 0 else 'heads'}, tiles), got {tuple(mask.shape)}")
-    return mask if mask.shape[2] <= 1 or mask.stride(2) == 1 else mask.contiguous()

@@ -145,7 +145,8 @@ def test_rotary_table_arguments():
 
 
 def test_overlaps():
-    from orthocache_gpu.rotary import overlaps
+    from orthocache_gpu._ops import ops
+    overlaps = ops().overlaps
     x = torch.zeros((4, 6, 8))
     assert not overlaps(x) and not overlaps(x.transpose(0, 2)) and not overlaps(x[:, ::2, 3:]) and not overlaps(x[:, :1])
     assert overlaps(x[:, :1].expand(4, 6, 8)) and overlaps(torch.as_strided(x, (3, 4), (2, 1)))
