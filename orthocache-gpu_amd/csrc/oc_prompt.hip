@@ -72,53 +72,121 @@ struct Sight {
   const int* tdoc;           // LDS: documents of the tile's 64 tokens
 };
 
-// Online-softmax update of one tile (as pf_softmax) with the scores changed:
-// c becomes 2^(z - m) for the tokens seen, 0 for the others.  CAP:
-// z = cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)).
+// The cap: a raw score c becomes tanh(k c), k = scale / cap.  float32 takes
+// tanhf.  The 16-bit kernels take y times a cubic in y^2 while |y| = |k c| is at
+// most kTanhFit (tanh(y) / y, fitted with a relative error of 5.5e-7 there), and
+// 1 - 2 / (1 + e^2y) with the hardware's exponential and reciprocal where a
+// score of the wave's tile is larger: six full-rate instructions against three
+// and two quarter-rate ones.
+constexpr float kTanhFit = 0.5f;
+constexpr float kTanh0 = 0.999999456f, kTanh1 = -0.333263178f, kTanh2 = 0.131902954f, kTanh3 = -0.0444021952f;
+
+template <int DT>
+__device__ __forceinline__ void cap_scores(f32x4 (&c)[4], float k) {
+  if constexpr (DT == OC_F32) {
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[tb][i] = tanhf(c[tb][i] * k);
+  } else {
+    float top = 0.f;
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[tb][i] *= k;
+        top = fmaxf(top, fabsf(c[tb][i]));
+      }
+    if (__builtin_amdgcn_ballot_w64(top > kTanhFit)) {
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          c[tb][i] = __builtin_fmaf(
+              -2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(c[tb][i] * (2.f * kLog2e))), 1.f);
+    } else {
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = c[tb][i], u = y * y;
+          c[tb][i] = y * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(kTanh3, u, kTanh2), u, kTanh1), u, kTanh0);
+        }
+    }
+  }
+}
+
+// What a head's scores go through: z = s (c - slope |i - j|) in base-2 units,
+// with c the raw score or its tanh, and s = pre.  Where pre is negative or next
+// to nothing, c is multiplied by it, and s is 1.
+constexpr float kSmallest = 1e-6f;
+struct Change {
+  float s;
+  float pre;    // cap log2(e) with a cap, else scale log2(e)
+  float k;      // scale / cap
+  float slope;  // the head's slope log2(e) / s
+};
+
+// Online-softmax update of one tile (as pf_softmax) with the scores changed: c
+// becomes 2^(z - m) for the tokens seen, 0 for the others.
 template <int DT, int D, bool CAP, bool BIAS>
-__device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16], f32x4 (&c)[4], float scale, float cap,
-                                               float slope2, const Sight& e, int tok0, bool full) {
+__device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16], f32x4 (&c)[4], const Change& h,
+                                               const Sight& e, int tok0, bool full) {
   float mt = -__builtin_inff();
+  if constexpr (CAP) cap_scores<DT>(c, h.k);
+  if (h.pre < kSmallest) {
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb) c[tb] *= h.pre;
+  }
   // the lane's place in the tile, formed from the thread index (lane =
   // threadIdx.x mod 64) so that nothing of it is kept across the tile loop
   int tx = threadIdx.x;
   asm volatile("" : "+v"(tx));
   const int r4 = (tx >> 2) & 12, x = tx & 15;
   const int rel = e.w_lo + x - tok0 - r4;  // distance of the lane's query to its first token of the tile
-  const float d0 = (float)rel;
-  const int pre = e.prefix - tok0 - r4;
-  int doc = 0;
-  if (e.qdoc && !full) doc = e.qdoc[x];
+  if constexpr (BIAS) {
+    const float d0 = (float)rel;
 #pragma unroll
-  for (int tb = 0; tb < 4; ++tb) {
-    int4 td = {0, 0, 0, 0};
-    if (e.qdoc && !full) td = *reinterpret_cast<const int4*>(e.tdoc + 16 * tb + r4);
-    const int tdv[4] = {td.x, td.y, td.z, td.w};
+    for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float z;
-      if constexpr (CAP) {
-        if constexpr (DT == OC_F32) {
-          z = cap * kLog2e * tanhf(c[tb][i] * scale / cap);
-        } else {
-          const float ex = __builtin_amdgcn_exp2f(c[tb][i] * (2.f * kLog2e * scale / cap));
-          z = __builtin_fmaf(-2.f * kLog2e * cap, __builtin_amdgcn_rcpf(1.f + ex), kLog2e * cap);
-        }
-      } else {
-        z = c[tb][i] * (scale * kLog2e);
-      }
-      if constexpr (BIAS) z = __builtin_fmaf(-slope2, fabsf(d0 - (float)(16 * tb + i)), z);
-      if (!full) {
+      for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(-h.slope, fabsf(d0 - (float)(16 * tb + i)), c[tb][i]);
+  }
+  if (full) {
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, c[tb][i]);
+  } else {
+    const int pre = e.prefix - tok0 - r4;
+    const bool docs = e.qdoc != nullptr;
+    int doc = 0;
+    if (docs) doc = e.qdoc[x];
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb) {
+      int4 td = {0, 0, 0, 0};
+      if (docs) td = *reinterpret_cast<const int4*>(e.tdoc + 16 * tb + r4);
+      const int tdv[4] = {td.x, td.y, td.z, td.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         const int d = rel - (16 * tb + i);
-        const bool ok = ((d >= 0 && d < e.window) || 16 * tb + i < pre) && tdv[i] == doc && doc >= 0;
-        z = ok ? z : -__builtin_inff();
+        // d in [0, window), both bounds in one comparison
+        const bool ok = ((unsigned)d < (unsigned)e.window || 16 * tb + i < pre) && tdv[i] == doc && doc >= 0;
+        c[tb][i] = ok ? c[tb][i] : -__builtin_inff();
+        mt = fmaxf(mt, c[tb][i]);
       }
-      c[tb][i] = z;
-      mt = fmaxf(mt, z);
     }
   }
+  float s = h.s;
+  mt *= s;
   mt = fmaxf(mt, xpair<16>(mt));
   mt = fmaxf(mt, xpair<32>(mt));
+  // Far from zero the maximum's rounding is no longer small against 1, and the
+  // fma below would see it: there the scores are rounded like the maximum.
+  if (__builtin_amdgcn_ballot_w64(fabsf(mt) > 16777216.f)) {
+#pragma unroll
+    for (int tb = 0; tb < 4; ++tb) c[tb] *= s;
+    s = 1.f;
+  }
   const bool move = mt > st.m + kPfSlack;
   if (__builtin_amdgcn_ballot_w64(move)) {
     const float mn = move ? mt : st.m;
@@ -133,7 +201,7 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
   for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float p = __builtin_amdgcn_exp2f(c[tb][i] - st.m);
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[tb][i], s, -st.m));
       ls += p;
       c[tb][i] = p;
     }
@@ -255,7 +323,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   __shared__ int bad_tile[2];  // the tile of each stage that holds V values which are not finite
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int wave = tid >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: so are the tests of what the wave sees
   // (batch, head) pairs and query blocks as in the prefill kernel: an eighth
   // of the pairs per XCD, longest causal windows first
   const int nbh = a.B * a.Hq;
@@ -316,7 +384,11 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   const char* kh = a.k + (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh;
   const char* vh = a.v + (int64_t)b * a.v_sb + (int64_t)kv * a.v_sh;
   const uint8_t* erow = a.evict ? a.evict + (int64_t)b * a.e_sb + (int64_t)kv * a.e_sh : nullptr;
-  const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+  Change change;
+  change.pre = (CAP ? a.cap : a.scale) * kLog2e;
+  change.s = change.pre < kSmallest ? 1.f : change.pre;
+  change.k = CAP ? a.scale / a.cap : 0.f;
+  change.slope = BIAS ? a.slopes[h] * kLog2e / change.s : 0.f;
 
   // the tiles of the workgroup, 64 at a time; of those, the ones whose
   // documents are all the wave's one document
@@ -371,7 +443,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
       f32x4 c[4];
       pf_logits<DT, D>(q, ck, lane, c);
       const Sight eye{w_lo, window, prefix, docs ? sqdoc + 16 * wave : nullptr, cd};
-      prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, a.scale, a.cap, slope2, eye, t * 64, full);
+      prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, change, eye, t * 64, full);
       if constexpr (ANY) prompt_pv_any<DT, D>(accp, c, cv, lane);
       else pf_pv<DT, D, false>(accp, c, cv, lane);
     };
@@ -381,12 +453,14 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
     if constexpr (L::STAGES == 2) {
       // the tile's documents go straight to LDS as well (past the last: 0, masked as no one sees those)
       auto fetch = [&](int t, char* nk, char* nv, int* nd) {
-        pf_fetch_lds<DT, D>(pa, kh, vh, t, tid, nk, nv);
+        int tf = tid;  // the loads' offsets formed for each tile, not kept in registers
+        asm volatile("" : "+v"(tf));
+        pf_fetch_lds<DT, D>(pa, kh, vh, t, tf, nk, nv);
         if (docs && wave == 0) {
           const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
               (void*)pf_uniform((const char*)docs), (short)0, __builtin_amdgcn_readfirstlane(a.Skv * 4), 0x00020000);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)nd, 4, 4 * (64 * t + lane),
-                                                   0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)nd, 4, 4 * (64 * t + lane), 0,
+                                                   0, 0);
         }
       };
       // what this thread staged of tile t's V, looked at once its loads have landed
@@ -411,7 +485,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
       };
       while (t < t_hi) {
         __syncthreads();  // stage s is complete; every wave is done with stage s ^ 1
-        if (!ANY && bad_tile[s] == t) return true;  // (uniform; no load is in flight)
+        if (!ANY && border(t) && bad_tile[s] == t) return true;  // (uniform; no load is in flight)
         const int tn = next_tile();
         const bool un = uniform;
         step(tn, stage_k(1 - s), stage_v(1 - s), sdoc[1 - s], stage_k(s), stage_v(s), sdoc[s]);
@@ -444,7 +518,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
       }
       while (t < t_hi) {
         __syncthreads();  // the stage is complete
-        if (!ANY && bad_tile[0] == t) return true;
+        if (!ANY && border(t) && bad_tile[0] == t) return true;
         const int tn = next_tile();
         const bool un = uniform;
         if (tn < t_hi) fetch(tn);  // in flight during this tile
