@@ -362,7 +362,8 @@ __device__ __forceinline__ void pf_logits(const PfQ<DT, D>& q, const char* sk, i
 // causal rows past the output tolerance.
 // float32: 16x16x4 steps over (tb, i), A = V[16tb + 4r + i][16nc + x], B =
 // c[tb][i], exact.
-template <int DT, int D, bool HILO = DT == OC_BF16>
+// PK: float16 pairs by one instruction (the same rounding).
+template <int DT, int D, bool HILO = DT == OC_BF16, bool PK = false>
 __device__ __forceinline__ void pf_pv(f32x4 (&acc)[D / 16], const f32x4 (&c)[4], const char* svb, int lane) {
   const int x = lane & 15;
   const int kg = lane >> 4;
@@ -398,6 +399,11 @@ __device__ __forceinline__ void pf_pv(f32x4 (&acc)[D / 16], const f32x4 (&c)[4],
             const __bf16 l0 = (__bf16)(pv[2 * e] - (float)h0), l1 = (__bf16)(pv[2 * e + 1] - (float)h1);
             blo[e] = (uint32_t)__builtin_bit_cast(uint16_t, l0) | ((uint32_t)__builtin_bit_cast(uint16_t, l1) << 16);
           }
+        } else if constexpr (PK) {
+          static_assert(!HILO, "pairs are rounded once");
+          typedef float f32x2 __attribute__((ext_vector_type(2)));
+          typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+          bhi[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{pv[2 * e], pv[2 * e + 1]}), f16x2));
         } else {
           const _Float16 h0 = (_Float16)pv[2 * e], h1 = (_Float16)pv[2 * e + 1];
           bhi[e] = (uint32_t)__builtin_bit_cast(uint16_t, h0) | ((uint32_t)__builtin_bit_cast(uint16_t, h1) << 16);

@@ -50,6 +50,14 @@ struct PromptArgs {
   int32_t o_vec;  // out rows 8-byte aligned
 };
 
+// The kernel's arguments, read again from memory where they are used: held
+// across the tile loop they would fill the scalar registers and push others out.
+__device__ __forceinline__ const PromptArgs __attribute__((address_space(4))) * prompt_args() {
+  auto p = (const PromptArgs __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 // the smallest and largest document of each 64-token tile: one wave a tile
 __global__ __launch_bounds__(256) void doc_range_kernel(const int32_t* docs, int64_t docs_sb, int n, int tiles, int all,
                                                         int2* out) {
@@ -68,7 +76,7 @@ __global__ __launch_bounds__(256) void doc_range_kernel(const int32_t* docs, int
 // What the wave's queries see: query x is at place w_lo + x.
 struct Sight {
   int w_lo, window, prefix;  // window: INT_MAX without one
-  const int* qdoc;           // LDS: documents of the wave's 16 queries, or null
+  const int* qdoc;           // LDS: documents of the wave's 16 queries; null where they need not be looked at
   const int* tdoc;           // LDS: documents of the tile's 64 tokens
 };
 
@@ -144,12 +152,24 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
   asm volatile("" : "+v"(tx));
   const int r4 = (tx >> 2) & 12, x = tx & 15;
   const int rel = e.w_lo + x - tok0 - r4;  // distance of the lane's query to its first token of the tile
+  // the bias: -slope (d0 - n) for the lane's token n of the tile, n = 16 tb + i.
+  // Where every token seen is at or before the query, its part in d0 is one
+  // offset for the lane's scores; only behind a prefix can one be after it.
+  float off = 0.f;
   if constexpr (BIAS) {
     const float d0 = (float)rel;
+    if (e.prefix <= tok0 || tok0 + 63 <= e.w_lo) {
+      off = h.slope * d0 * h.s;
 #pragma unroll
-    for (int tb = 0; tb < 4; ++tb)
+      for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(-h.slope, fabsf(d0 - (float)(16 * tb + i)), c[tb][i]);
+        for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(h.slope, (float)(16 * tb + i), c[tb][i]);
+    } else {
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(-h.slope, fabsf(d0 - (float)(16 * tb + i)), c[tb][i]);
+    }
   }
   if (full) {
 #pragma unroll
@@ -158,34 +178,44 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
       for (int i = 0; i < 4; ++i) mt = fmaxf(mt, c[tb][i]);
   } else {
     const int pre = e.prefix - tok0 - r4;
-    const bool docs = e.qdoc != nullptr;
-    int doc = 0;
-    if (docs) doc = e.qdoc[x];
+    if (!e.qdoc && e.prefix <= tok0) {  // the causal border and the window alone
 #pragma unroll
-    for (int tb = 0; tb < 4; ++tb) {
-      int4 td = {0, 0, 0, 0};
-      if (docs) td = *reinterpret_cast<const int4*>(e.tdoc + 16 * tb + r4);
-      const int tdv[4] = {td.x, td.y, td.z, td.w};
+      for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = rel - (16 * tb + i);
-        // d in [0, window), both bounds in one comparison
-        const bool ok = ((unsigned)d < (unsigned)e.window || 16 * tb + i < pre) && tdv[i] == doc && doc >= 0;
-        c[tb][i] = ok ? c[tb][i] : -__builtin_inff();
-        mt = fmaxf(mt, c[tb][i]);
+        for (int i = 0; i < 4; ++i) {
+          // the distance in [0, window), both bounds in one comparison
+          c[tb][i] = (unsigned)(rel - (16 * tb + i)) < (unsigned)e.window ? c[tb][i] : -__builtin_inff();
+          mt = fmaxf(mt, c[tb][i]);
+        }
+    } else {
+      const int doc = e.qdoc ? e.qdoc[x] : 0;
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb) {
+        int4 td = {0, 0, 0, 0};
+        if (e.qdoc) td = *reinterpret_cast<const int4*>(e.tdoc + 16 * tb + r4);
+        const int tdv[4] = {td.x, td.y, td.z, td.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = ((unsigned)(rel - (16 * tb + i)) < (unsigned)e.window || 16 * tb + i < pre) && tdv[i] == doc && doc >= 0;
+          c[tb][i] = ok ? c[tb][i] : -__builtin_inff();
+          mt = fmaxf(mt, c[tb][i]);
+        }
       }
     }
   }
   float s = h.s;
-  mt *= s;
+  mt = __builtin_fmaf(mt, s, -off);
   mt = fmaxf(mt, xpair<16>(mt));
   mt = fmaxf(mt, xpair<32>(mt));
   // Far from zero the maximum's rounding is no longer small against 1, and the
   // fma below would see it: there the scores are rounded like the maximum.
   if (__builtin_amdgcn_ballot_w64(fabsf(mt) > 16777216.f)) {
 #pragma unroll
-    for (int tb = 0; tb < 4; ++tb) c[tb] *= s;
+    for (int tb = 0; tb < 4; ++tb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(c[tb][i], s, -off);
     s = 1.f;
+    off = 0.f;
   }
   const bool move = mt > st.m + kPfSlack;
   if (__builtin_amdgcn_ballot_w64(move)) {
@@ -197,11 +227,12 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
     for (int nc = 0; nc < D / 16; ++nc) acc[nc] *= alpha;
   }
   float ls = 0.f;
+  off += st.m;
 #pragma unroll
   for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[tb][i], s, -st.m));
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[tb][i], s, -off));
       ls += p;
       c[tb][i] = p;
     }
@@ -304,6 +335,48 @@ __device__ __forceinline__ bool not_finite(const uint4& u) {
   return bad;
 }
 
+// A thread's part of the loads of pf_fetch_lds: its row and 16-byte piece of K
+// and of V in the tile's first 512 pieces.  The others are whole rows of 512
+// pieces further, in K and V as in LDS (the layouts repeat there), so that one
+// offset each is all there is to keep.
+template <int DT, int D>
+struct PromptFetch {
+  using L = PfTile<DT, D>;
+  static constexpr int STEP = kPfThreads / L::LPT;  // rows per 512 pieces
+  static_assert(L::NL == 1 || (STEP % 32 == 0 && STEP / L::RB % L::LPT == 0), "layouts that repeat every STEP rows");
+  int k, v;
+
+  __device__ static __forceinline__ PromptFetch of(const PrefillArgs& a, int tid) {
+    const int r = tid / L::LPT, c = tid % L::LPT;
+    return {r * (int)a.k_ss + 16 * (c ^ L::swz(r)),
+            DT == OC_F32 ? r * (int)a.v_ss + 16 * c : pf_vtok(r) * (int)a.v_ss + 16 * (c ^ (2 * L::vswz(r)))};
+  }
+
+  // tile t straight to LDS, rows at or past kv_len as zeros; by the first wave
+  // the tile's documents too (past the last: 0, of places that no one sees)
+  __device__ __forceinline__ void operator()(const PrefillArgs& a, const char* kh, const char* vh, const int32_t* docs,
+                                             int t, int tid, char* nk, char* nv, int* nd) const {
+    t = __builtin_amdgcn_readfirstlane(t);
+    const int wbase = __builtin_amdgcn_readfirstlane(tid & ~63);
+#pragma unroll
+    for (int j = 0; j < L::NL; ++j) {
+      const int row = 64 * t + STEP * j, n = max(min(a.Skv - row, 64 - STEP * j), 0);
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)pf_uniform(kh + (int64_t)row * (int)a.k_ss), (short)0, __builtin_amdgcn_readfirstlane(n * (int)a.k_ss), 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)pf_uniform(vh + (int64_t)row * (int)a.v_ss), (short)0, __builtin_amdgcn_readfirstlane(n * (int)a.v_ss), 0x00020000);
+      pf_load_lds16(rk, nk + 16 * (wbase + kPfThreads * j), k);
+      pf_load_lds16(rv, nv + 16 * (wbase + kPfThreads * j), v);
+    }
+    if (docs && wbase == 0) {
+      const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)pf_uniform((const char*)docs), (short)0, __builtin_amdgcn_readfirstlane(a.Skv * 4), 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)nd, 4,
+                                               4 * (64 * t + (int)__lane_id()), 0, 0, 0);
+    }
+  }
+};
+
 __device__ __forceinline__ int wave_min_i(int v) {
   for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
   return v;
@@ -317,10 +390,16 @@ template <int DT, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT == OC_F32 && D == 128 ? 1 : 4))) void prompt_kernel(
     const PromptArgs a) {
   using L = PfTile<DT, D>;
-  __shared__ __attribute__((aligned(16))) char sh[L::LDS];
-  __shared__ __attribute__((aligned(16))) int sdoc[2][64];
-  __shared__ int sqdoc[kPfRows];
-  __shared__ int bad_tile[2];  // the tile of each stage that holds V values which are not finite
+  // One LDS array for all: with several, the compiler takes the loads into one
+  // stage for writes to the other, and waits for them before each tile's reads.
+  // Behind the stages: the documents of the two stages' tokens and of the
+  // workgroup's queries, their ranges, and the tile of each stage that holds V
+  // values which are not finite.
+  __shared__ __attribute__((aligned(16))) char sh[L::LDS + 4 * (2 * 64 + kPfRows + 4 * kPfWaves + 2)];
+  int* const sdoc0 = reinterpret_cast<int*>(sh + L::LDS);
+  int* const sqdoc = sdoc0 + 2 * 64;
+  int* const swave = sqdoc + kPfRows;  // four of each wave: documents of its queries, and of the workgroup's
+  int* const bad_tile = swave + 4 * kPfWaves;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // scalar: so are the tests of what the wave sees
@@ -351,19 +430,18 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
     const int p = s + off;
     return s < a.Sq && p >= 0 ? docs[p] : -1;
   };
-  // documents of the wave's queries, and of the workgroup's: [least, most] of those that are not negative
-  int wd0 = 0, wd1 = 0, gd0 = 0, gd1 = 0;
   if (docs) {
+    // documents of the wave's queries, and of the workgroup's: the least and the most of those that are not negative
     const int doc = doc_at(pos0 + x);
-    if (lane < 16) sqdoc[16 * wave + lane] = doc;  // read by this wave alone
+    if (lane < 16) sqdoc[16 * wave + lane] = doc;  // read by this wave alone, like swave
     const int d0 = doc_at(qb * kPfRows + lane), d1 = doc_at(qb * kPfRows + 64 + lane);
     auto least = [](int d) { return d < 0 ? INT_MAX : d; };
-    wd0 = wave_min_i(least(doc)), wd1 = wave_max_i(doc);
-    // (a wave with a query past Sq or of no document is not uniform)
-    if (__builtin_amdgcn_ballot_w64(doc < 0 && pos0 + x < a.Sq)) wd1 = INT_MAX;
-    gd0 = wave_min_i(min(least(d0), least(d1))), gd1 = wave_max_i(max(d0, d1));
+    const int wd0 = wave_min_i(least(doc)), wd1 = wave_max_i(doc);
+    const int gd0 = wave_min_i(min(least(d0), least(d1))), gd1 = wave_max_i(max(d0, d1));
+    // (a wave with a query of no document is not of one document)
+    const bool none = __builtin_amdgcn_ballot_w64(doc < 0 && pos0 + x < a.Sq) != 0;
+    if (lane == 0) *reinterpret_cast<int4*>(swave + 4 * wave) = int4{wd0, none ? INT_MAX : wd1, gd0, gd1};
   }
-  const int2* ranges = a.docs ? a.ranges + (int64_t)b * ((a.Skv + 63) / 64) : nullptr;
   // places of the wave's first and last query, and of the workgroup's
   const int w_lo = pos0 + off, w_hi = min(pos0 + 15, a.Sq - 1) + off;
   const int g_lo = qb * kPfRows + off, g_hi = min(qb * kPfRows + kPfRows - 1, a.Sq - 1) + off;
@@ -383,46 +461,59 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   pf_load_q<DT, D>(pa, a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh, pos0, lane, q);
   const char* kh = a.k + (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh;
   const char* vh = a.v + (int64_t)b * a.v_sb + (int64_t)kv * a.v_sh;
-  const uint8_t* erow = a.evict ? a.evict + (int64_t)b * a.e_sb + (int64_t)kv * a.e_sh : nullptr;
   Change change;
   change.pre = (CAP ? a.cap : a.scale) * kLog2e;
   change.s = change.pre < kSmallest ? 1.f : change.pre;
   change.k = CAP ? a.scale / a.cap : 0.f;
   change.slope = BIAS ? a.slopes[h] * kLog2e / change.s : 0.f;
 
-  // the tiles of the workgroup, 64 at a time; of those, the ones whose
-  // documents are all the wave's one document
+  // The tiles of the workgroup, 64 at a time, and what is true of each: that the
+  // wave needs it, that all its queries see all of it (documents apart), that
+  // its documents are all the wave's one document, and that some query of the
+  // workgroup does not see all of it.
   int word = 0;
-  uint64_t bits = 0, ubits = 0;
+  uint64_t bits = 0, w_need = 0, w_whole = 0, w_one = 0, g_border = 0;
   auto load_word = [&](int w) {
+    const auto ap = prompt_args();
     const int t = 64 * w + (int)__lane_id();
     bool keep = t < t_hi && needed(t, g_lo, g_hi);
-    if (erow) keep = keep && !(t < a.T && erow[min(t, a.T - 1)]);
+    if (ap->evict) {
+      const uint8_t* row = ap->evict + (int64_t)b * ap->e_sb + (int64_t)kv * ap->e_sh;
+      keep = keep && !(t < ap->T && row[min(t, ap->T - 1)]);
+    }
     bool one = true;
     if (docs) {
-      const int2 d = ranges[min(t, (a.Skv - 1) / 64)];
-      keep = keep && d.y >= gd0 && d.x <= gd1;
-      one = d.x == d.y && d.x == wd0 && d.x == wd1;
+      const int last = (ap->Skv - 1) / 64;
+      const int2 d = ap->ranges[(int64_t)b * (last + 1) + min(t, last)];
+      const int4 q = *reinterpret_cast<const int4*>(swave + 4 * wave);
+      keep = keep && d.y >= q.z && d.x <= q.w;
+      one = d.x == d.y && d.x == q.x && d.x == q.y;
     }
     bits = __builtin_amdgcn_ballot_w64(keep);
-    ubits = __builtin_amdgcn_ballot_w64(one);
+    w_need = __builtin_amdgcn_ballot_w64(active && needed(t, w_lo, w_hi));
+    w_whole = __builtin_amdgcn_ballot_w64(whole(t, w_lo, w_hi));
+    w_one = __builtin_amdgcn_ballot_w64(one);
+    g_border = __builtin_amdgcn_ballot_w64(docs || !whole(t, g_lo, g_hi));
   };
-  bool uniform = true;  // of the tile last taken
+  struct Tile {
+    int t;  // t_hi when there is none
+    bool need, whole, one, border;
+  };
   auto next_tile = [&]() {
     while (bits == 0) {
-      if (64 * ++word >= t_hi) return t_hi;
+      if (64 * ++word >= t_hi) return Tile{t_hi, false, false, false, false};
       load_word(word);
     }
-    const int t = 64 * word + __builtin_ctzll(bits);
-    uniform = ubits & bits & -bits;
+    const uint64_t b = bits & -bits;
+    const Tile r{64 * word + __builtin_ctzll(bits), (w_need & b) != 0, (w_whole & b) != 0, (w_one & b) != 0, (g_border & b) != 0};
     bits &= bits - 1;
-    return t;
+    return r;
   };
+
   PfState st;
   f32x4 accp[D / 16];
   auto stage_k = [&](int s) { return sh + s * 2 * L::KV; };
   auto stage_v = [&](int s) { return sh + s * 2 * L::KV + L::KV; };
-  auto border = [&](int t) { return docs || !whole(t, g_lo, g_hi); };  // uniform over the workgroup
   // One pass over the tiles.  The first takes V to be finite where it matters
   // and gives up (true) at the first border tile whose V is not; the second
   // then starts over with prompt_pv_any.  (Both forms of p.V in one loop need
@@ -430,70 +521,60 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   auto pass = [&](auto any_c) -> bool {
     constexpr bool ANY = decltype(any_c)::value;
     word = 0;
-    bits = ubits = 0;
+    bits = 0;
     if (t_hi > 0) load_word(0);
     st = PfState{kNoScore, 0.f, 0.f, 0};
 #pragma unroll
     for (int nc = 0; nc < D / 16; ++nc) accp[nc] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (tid < 2) bad_tile[tid] = -1;
-    auto compute = [&](int t, bool uni, const char* __restrict__ ck, const char* __restrict__ cv,
-                       const int* __restrict__ cd) {
-      if (!active || !needed(t, w_lo, w_hi)) return;
-      const bool full = uni && whole(t, w_lo, w_hi);
-      f32x4 c[4];
-      pf_logits<DT, D>(q, ck, lane, c);
-      const Sight eye{w_lo, window, prefix, docs ? sqdoc + 16 * wave : nullptr, cd};
-      prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, change, eye, t * 64, full);
-      if constexpr (ANY) prompt_pv_any<DT, D>(accp, c, cv, lane);
-      else pf_pv<DT, D, false>(accp, c, cv, lane);
-    };
-    int t = next_tile();
-    bool uni = uniform;
+    Tile cur = next_tile();
     __syncthreads();  // bad_tile
     if constexpr (L::STAGES == 2) {
-      // the tile's documents go straight to LDS as well (past the last: 0, masked as no one sees those)
-      auto fetch = [&](int t, char* nk, char* nv, int* nd) {
-        int tf = tid;  // the loads' offsets formed for each tile, not kept in registers
-        asm volatile("" : "+v"(tf));
-        pf_fetch_lds<DT, D>(pa, kh, vh, t, tf, nk, nv);
-        if (docs && wave == 0) {
-          const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)pf_uniform((const char*)docs), (short)0, __builtin_amdgcn_readfirstlane(a.Skv * 4), 0x00020000);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rd, (__attribute__((address_space(3))) void*)nd, 4, 4 * (64 * t + lane), 0,
-                                                   0, 0);
-        }
-      };
-      // what this thread staged of tile t's V, looked at once its loads have landed
-      auto landed = [&](int t, int s) {
-        if (ANY || !border(t)) return;
+      // what this thread staged of a border tile's V, looked at once its loads have landed
+      auto landed = [&](const Tile& n, int s) {
+        if (ANY || !n.border || n.t >= t_hi) return;
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < L::NL; ++j)
           bad |= not_finite<DT>(*reinterpret_cast<const uint4*>(stage_v(s) + 16 * (tid + kPfThreads * j)));
-        if (bad) bad_tile[s] = t;
+        if (bad) bad_tile[s] = n.t;
       };
-      if (t < t_hi) fetch(t, stage_k(0), stage_v(0), sdoc[0]);
+      const auto first = PromptFetch<DT, D>::of(pa, tid);
+      if (cur.t < t_hi) first(pa, kh, vh, docs, cur.t, tid, stage_k(0), stage_v(0), sdoc0);
       __builtin_amdgcn_s_waitcnt(0);
-      if (t < t_hi) landed(t, 0);
+      landed(cur, 0);
       int s = 0;
       // the stages are restrict parameters, as in the prefill kernel: no wait for
       // the loads into one before the reads of the other
-      auto step = [&](int tn, char* __restrict__ nk, char* __restrict__ nv, int* __restrict__ nd,
+      auto step = [&](const Tile& n, char* __restrict__ nk, char* __restrict__ nv, int* __restrict__ nd,
                       const char* __restrict__ ck, const char* __restrict__ cv, const int* __restrict__ cd) {
-        if (tn < t_hi) fetch(tn, nk, nv, nd);
-        compute(t, uni, ck, cv, cd);
+        if (n.t < t_hi) {
+          if constexpr (CAP || BIAS) {
+            int tf = tid;  // the offsets formed again: two registers less across the tile
+            asm volatile("" : "+v"(tf));
+            PromptFetch<DT, D>::of(pa, tf)(pa, kh, vh, docs, n.t, tid, nk, nv, nd);
+          } else {
+            first(pa, kh, vh, docs, n.t, tid, nk, nv, nd);
+          }
+        }
+        if (cur.need) {
+          f32x4 c[4];
+          pf_logits<DT, D>(q, ck, lane, c);
+          const Sight eye{w_lo, window, prefix, docs && !cur.one ? sqdoc + 16 * wave : nullptr, cd};
+          prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, change, eye, cur.t * 64, cur.whole && cur.one);
+          if constexpr (ANY) prompt_pv_any<DT, D>(accp, c, cv, lane);
+          else pf_pv<DT, D, false, true>(accp, c, cv, lane);
+        }
       };
-      while (t < t_hi) {
+      while (cur.t < t_hi) {
         __syncthreads();  // stage s is complete; every wave is done with stage s ^ 1
-        if (!ANY && border(t) && bad_tile[s] == t) return true;  // (uniform; no load is in flight)
-        const int tn = next_tile();
-        const bool un = uniform;
-        step(tn, stage_k(1 - s), stage_v(1 - s), sdoc[1 - s], stage_k(s), stage_v(s), sdoc[s]);
+        if (!ANY && cur.border && bad_tile[s] == cur.t) return true;  // (uniform; no load is in flight)
+        const Tile n = next_tile();
+        step(n, stage_k(1 - s), stage_v(1 - s), sdoc0 + 64 * (1 - s), stage_k(s), stage_v(s), sdoc0 + 64 * s);
         __builtin_amdgcn_s_waitcnt(0);
         s = 1 - s;
-        if (tn < t_hi) landed(tn, s);
-        t = tn;
-        uni = un;
+        landed(n, s);
+        cur = n;
       }
     } else {
       // one stage (float32, head_dim 128): the next tile waits in registers
@@ -503,30 +584,35 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
         pf_fetch<DT, D>(pa, kh, vh, t, tid, reg);
         if (docs && wave == 0) dn = docs[min(64 * t + lane, a.Skv - 1)];
       };
-      auto stash = [&](int t) {
+      auto stash = [&](const Tile& n) {
         pf_stash<DT, D>(reg, tid, stage_k(0), stage_v(0));
-        if (docs && wave == 0) sdoc[0][lane] = dn;
-        if (ANY || !border(t)) return;
+        if (docs && wave == 0) sdoc0[lane] = dn;
+        if (ANY || !n.border) return;
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < L::NL; ++j) bad |= not_finite<DT>(reg.v[j]);
-        if (bad) bad_tile[0] = t;
+        if (bad) bad_tile[0] = n.t;
       };
-      if (t < t_hi) {
-        fetch(t);
-        stash(t);
+      if (cur.t < t_hi) {
+        fetch(cur.t);
+        stash(cur);
       }
-      while (t < t_hi) {
+      while (cur.t < t_hi) {
         __syncthreads();  // the stage is complete
-        if (!ANY && border(t) && bad_tile[0] == t) return true;
-        const int tn = next_tile();
-        const bool un = uniform;
-        if (tn < t_hi) fetch(tn);  // in flight during this tile
-        compute(t, uni, stage_k(0), stage_v(0), sdoc[0]);
+        if (!ANY && cur.border && bad_tile[0] == cur.t) return true;
+        const Tile n = next_tile();
+        if (n.t < t_hi) fetch(n.t);  // in flight during this tile
+        if (cur.need) {
+          f32x4 c[4];
+          pf_logits<DT, D>(q, stage_k(0), lane, c);
+          const Sight eye{w_lo, window, prefix, docs && !cur.one ? sqdoc + 16 * wave : nullptr, sdoc0};
+          prompt_softmax<DT, D, CAP, BIAS>(st, accp, c, change, eye, cur.t * 64, cur.whole && cur.one);
+          if constexpr (ANY) prompt_pv_any<DT, D>(accp, c, stage_v(0), lane);
+          else pf_pv<DT, D, false, true>(accp, c, stage_v(0), lane);
+        }
         __syncthreads();  // the stage is free again
-        if (tn < t_hi) stash(tn);
-        t = tn;
-        uni = un;
+        if (n.t < t_hi) stash(n);
+        cur = n;
       }
     }
     return false;
@@ -544,8 +630,9 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   int tl = threadIdx.x;  // formed after the loop, as in the prefill kernel
   asm volatile("" : "+v"(tl));
   const int qpos = pos0 + (tl & 15), r = (tl >> 4) & 3;
-  if (qpos < a.Sq) {
-    char* orow = a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)qpos * a.o_ss;
+  const auto ap = prompt_args();
+  if (qpos < ap->Sq) {
+    char* orow = ap->out + (int64_t)b * ap->o_sb + (int64_t)h * ap->o_sh + (int64_t)qpos * ap->o_ss;
 #pragma unroll
     for (int nc = 0; nc < D / 16; ++nc) {
       const int col = 16 * nc + 4 * r;
@@ -555,7 +642,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
       } else {
         const uint2 w = {pf_pack<DT>(accp[nc][0] * inv, accp[nc][1] * inv),
                          pf_pack<DT>(accp[nc][2] * inv, accp[nc][3] * inv)};
-        if (a.o_vec) {
+        if (ap->o_vec) {
           *reinterpret_cast<uint2*>(orow + 2 * col) = w;
         } else {
           uint16_t* o = reinterpret_cast<uint16_t*>(orow + 2 * col);
