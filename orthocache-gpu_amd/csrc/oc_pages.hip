@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
 }
 
 // Workgroups: n_out rows of the new tables, n_in old rows whose blocks change
-// holders, then (child, layer) pairs that copy a last block's K and V.
+// holders, then (child, layer, K or V) triples that copy a last block.
 __global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const ForkArgs a) {
   const int tid = threadIdx.x;
   const bool ok = *a.plan == 0;
@@ -239,37 +239,47 @@ __global__ __launch_bounds__(kRowThreads) void fork_rows_kernel(const ForkArgs a
     return;
   }
   g -= a.n_in;
-  const int i = (int)(g / a.layers), layer = (int)(g % a.layers);
+  const int i = (int)(g / (2 * a.layers));
+  const int layer = (int)(g % (2 * a.layers)) >> 1;
+  const bool is_v = g & 1;
   if (!(a.have[i] & kFlag)) return;
   const int s = a.parents ? a.parents[i] : i;
   const int64_t n = fork_len(a, s);
   const int part = (int)(n & (bs - 1));
   const int64_t src = a.tables[s * a.bt_stride + (n >> a.block_log2)];
   const int64_t dst = a.free[a.take[i]];
-  // rows of row_bytes (a multiple of 16: uint4, else of 4 or 1), part of them a
-  // head; K and V in turn
-  auto copy = [&](char* pool, int64_t sl, int64_t sb, int64_t sh, int64_t ss, auto unit) {
+  const int64_t sb = is_v ? a.v_sb : a.k_sb, sh = is_v ? a.v_sh : a.k_sh, ss = is_v ? a.v_ss : a.k_ss;
+  char* pool = (is_v ? a.vc + layer * a.v_sl : a.kc + layer * a.k_sl);
+  // rows of row_bytes, part of them a head, in units of 16 bytes where
+  // everything is a multiple of that, else of one; eight units a thread are
+  // read before the first is written
+  auto copy = [&](auto unit) {
     using U = decltype(unit);
-    char* from = pool + layer * sl + src * sb;
-    char* to = pool + layer * sl + dst * sb;
+    constexpr int AHEAD = 8;
+    const char* from = pool + src * sb;
+    char* to = pool + dst * sb;
     const int upr = a.row_bytes / (int)sizeof(U);
-    const int perhead = part * upr;
-    for (int u = tid; u < a.heads * perhead; u += kRowThreads) {
-      const int h = u / perhead, r = u - h * perhead;
-      const int t = r / upr, c = r - t * upr;
-      const int64_t off = h * sh + t * ss + c * (int64_t)sizeof(U);
-      *reinterpret_cast<U*>(to + off) = *reinterpret_cast<const U*>(from + off);
+    const int perhead = part * upr, all = a.heads * perhead;
+    for (int u0 = tid; u0 < all; u0 += AHEAD * kRowThreads) {
+      int64_t off[AHEAD];
+      U w[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int u = min(u0 + e * kRowThreads, all - 1);
+        const int h = u / perhead, r = u - h * perhead;
+        const int t = r / upr, c = r - t * upr;
+        off[e] = h * sh + t * ss + c * (int64_t)sizeof(U);
+        w[e] = *reinterpret_cast<const U*>(from + off[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e)
+        if (u0 + e * kRowThreads < all) *reinterpret_cast<U*>(to + off[e]) = w[e];
     }
   };
-  const int64_t odd = (int64_t)(uintptr_t)a.kc | (int64_t)(uintptr_t)a.vc | a.k_sl | a.k_sb | a.k_sh | a.k_ss | a.v_sl |
-                      a.v_sb | a.v_sh | a.v_ss | a.row_bytes;
-  if (odd % 16 == 0) {
-    copy(a.kc, a.k_sl, a.k_sb, a.k_sh, a.k_ss, uint4{});
-    copy(a.vc, a.v_sl, a.v_sb, a.v_sh, a.v_ss, uint4{});
-  } else {
-    copy(a.kc, a.k_sl, a.k_sb, a.k_sh, a.k_ss, uint8_t{});
-    copy(a.vc, a.v_sl, a.v_sb, a.v_sh, a.v_ss, uint8_t{});
-  }
+  const int64_t odd = (int64_t)(uintptr_t)pool | sb | sh | ss | a.row_bytes;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if (odd % 16 == 0) copy(u32x4{});
+  else copy(uint8_t{});
 }
 
 struct EvictArgs {
@@ -317,15 +327,27 @@ __global__ __launch_bounds__(kRowThreads) void evict_rows_kernel(const EvictArgs
   int base = 0, left = 0;  // kept tiles so far; blocks written so far
   for (int t0 = 0; t0 < tiles; t0 += kRowThreads) {
     const int t = t0 + tid;
-    bool gone = t < whole && t < a.cols;
-    for (int h = 0; h < a.heads && gone; ++h) gone = e[h * a.e_sh + t] != 0;
+    // the tile's flags of every head and its first blocks, read at once
+    const bool may = t < whole && t < a.cols;
+    constexpr int HELD = 8;
+    int ids[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) ids[j] = t < tiles && j < per && t * per + j < blocks ? row[t * per + j] : -1;
+    bool gone = may;
+    if (may)
+      for (int h0 = 0; h0 < a.heads; h0 += HELD) {
+        uint8_t f[HELD];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) f[h] = e[min(h0 + h, a.heads - 1) * a.e_sh + t];
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) gone = gone && f[h] != 0;
+      }
     const bool kept = t < tiles && !gone;
     int total;
     const int at = base + block_excl_scan<kRowThreads>(kept ? 1 : 0, scan, total);
     if (t < tiles) {
       if (kept) map[at] = t;
-      for (int j = 0; j < per && t * per + j < blocks; ++j) {
-        int id = row[t * per + j];
+      auto put = [&](int j, int id) {
         const bool good = id >= 0 && id < a.num_blocks;
         if (!good) {
           atomicOr(a.status, OC_PAGES_BAD_BLOCK);
@@ -333,7 +355,11 @@ __global__ __launch_bounds__(kRowThreads) void evict_rows_kernel(const EvictArgs
         }
         if (kept) out[at * per + j] = id;
         else if (good) atomicAdd(a.out_refs + id, -1);
-      }
+      };
+#pragma unroll
+      for (int j = 0; j < HELD; ++j)
+        if (j < per && t * per + j < blocks) put(j, ids[j]);
+      for (int j = HELD; j < per && t * per + j < blocks; ++j) put(j, row[t * per + j]);
     }
     base += total;
   }
@@ -407,7 +433,7 @@ extern "C" int oc_fork_pages(const oc_fork_params* p, void* stream) {
   a.free = a.count + p->num_seqs;
   a.free_cap = (int32_t)fork_free_cap(p);
   const int64_t copiers = std::min<int64_t>((p->num_blocks + kPlanThreads - 1) / kPlanThreads, 256);
-  const int64_t blocks = (int64_t)p->num_children + p->num_seqs + (int64_t)p->num_children * p->layers;
+  const int64_t blocks = (int64_t)p->num_children + p->num_seqs + 2 * (int64_t)p->num_children * p->layers;
   if (blocks > 0x7FFFFFFF) return fail(OC_ERR_UNSUPPORTED, "too many layers");
   const hipStream_t s = (hipStream_t)stream;
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1 + (unsigned)copiers), dim3(kPlanThreads), 0, s, a);

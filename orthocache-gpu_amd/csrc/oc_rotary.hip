@@ -99,43 +99,66 @@ struct RowVecs {
   __device__ static int count(int rot, int d) { return turned(rot) + (d - rot) / N; }
 };
 
-// vector u of one row: sc holds the row's (cos, sin) pairs
+// A vector on its way: read, then turned and stored.  Two are in flight per
+// thread, so that a row of 16-byte vectors fills memory's latency like one of
+// 32-byte pairs does.
 template <int DT, bool VEC, bool INTER>
-__device__ __forceinline__ void turn_vec(const char* src, char* dst, int dst_dtype, int dst_es, float div, int u,
-                                         int rot, const float2* sc) {
+struct TurnVec {
   using R = RowVecs<DT, VEC, INTER>;
-  const int nt = R::turned(rot);
-  if (u >= nt) {
-    const int c = rot + (u - nt) * R::N;
-    float f[R::N];
-    load_n<DT, R::N>(src + c * R::ES, f);
-    store_n<R::N>(dst + c * dst_es, dst_dtype, div, f);
-  } else if constexpr (INTER) {
-    const int c = u * R::NP;
-    float f[R::NP], o[R::NP];
-    load_n<DT, R::NP>(src + c * R::ES, f);
-#pragma unroll
-    for (int i = 0; i < R::NP / 2; ++i) {
-      const float2 t = sc[c / 2 + i];
-      o[2 * i] = f[2 * i] * t.x - f[2 * i + 1] * t.y;
-      o[2 * i + 1] = f[2 * i + 1] * t.x + f[2 * i] * t.y;
+  float x0[R::NP], x1[INTER ? 1 : R::N];
+  char* dst;        // of the row
+  const float2* sc; // the token's (cos, sin) pairs
+  float div;
+  int u, rot, dtype, es;
+
+  // vector u of the row at src, into x0 and x1
+  __device__ __forceinline__ void read(const char* src) {
+    const int nt = R::turned(rot);
+    if constexpr (INTER && !VEC) {
+      if (u >= nt) {
+        x0[0] = load_scalar(src + (rot + u - nt) * R::ES, DT);
+        x0[1] = 0.f;
+      } else {
+        load_n<DT, 2>(src + 2 * u * R::ES, x0);
+      }
+    } else {
+      load_n<DT, R::N>(src + (u >= nt ? rot + (u - nt) * R::N : u * R::N) * R::ES, x0);
+      if constexpr (!INTER)
+        if (u < nt) load_n<DT, R::N>(src + (rot / 2 + u * R::N) * R::ES, x1);
     }
-    store_n<R::NP>(dst + c * dst_es, dst_dtype, div, o);
-  } else {
-    const int c = u * R::N, h = rot / 2;
-    float x0[R::N], x1[R::N], o0[R::N], o1[R::N];
-    load_n<DT, R::N>(src + c * R::ES, x0);
-    load_n<DT, R::N>(src + (h + c) * R::ES, x1);
-#pragma unroll
-    for (int i = 0; i < R::N; ++i) {
-      const float2 t = sc[c + i];
-      o0[i] = x0[i] * t.x - x1[i] * t.y;
-      o1[i] = x1[i] * t.x + x0[i] * t.y;
-    }
-    store_n<R::N>(dst + c * dst_es, dst_dtype, div, o0);
-    store_n<R::N>(dst + (h + c) * dst_es, dst_dtype, div, o1);
   }
-}
+
+  __device__ __forceinline__ void finish() const {
+    const int nt = R::turned(rot);
+    if (u >= nt) {
+      float o[R::N];
+#pragma unroll
+      for (int i = 0; i < R::N; ++i) o[i] = x0[i];
+      store_n<R::N>(dst + (rot + (u - nt) * R::N) * es, dtype, div, o);
+    } else if constexpr (INTER) {
+      const int c = u * R::NP;
+      float o[R::NP];
+#pragma unroll
+      for (int i = 0; i < R::NP / 2; ++i) {
+        const float2 t = sc[c / 2 + i];
+        o[2 * i] = x0[2 * i] * t.x - x0[2 * i + 1] * t.y;
+        o[2 * i + 1] = x0[2 * i + 1] * t.x + x0[2 * i] * t.y;
+      }
+      store_n<R::NP>(dst + c * es, dtype, div, o);
+    } else {
+      const int c = u * R::N;
+      float o0[R::N], o1[R::N];
+#pragma unroll
+      for (int i = 0; i < R::N; ++i) {
+        const float2 t = sc[c + i];
+        o0[i] = x0[i] * t.x - x1[i] * t.y;
+        o1[i] = x1[i] * t.x + x0[i] * t.y;
+      }
+      store_n<R::N>(dst + c * es, dtype, div, o0);
+      store_n<R::N>(dst + (rot / 2 + c) * es, dtype, div, o1);
+    }
+  }
+};
 
 // (cos, sin) of position n's pair, times scale; the angle in turns, float64
 __device__ __forceinline__ float2 angle_of(int64_t n, double f, float scale, bool backward) {
@@ -150,6 +173,20 @@ __device__ __forceinline__ int64_t position_at(const void* p, int is64, int64_t 
   return is64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
 }
 
+// Division of 0 <= n < 2^31 by a number fixed for the launch, as a high product
+// and a shift (the compiler's own takes some 40 instructions, and a vector needs
+// three: the 4762-token chunks into fp8 pages went from 36 to 33.5 us).
+struct Div {
+  uint32_t mul, shift;
+  Div() = default;
+  explicit Div(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
+};
+
 // strides in bytes
 struct RotArgs {
   const char* x[2];
@@ -161,6 +198,7 @@ struct RotArgs {
   int64_t pos_sb;
   const double* inv_freq;
   float scale;
+  Div by_nu, by_rows, by_half;  // vectors of a row, rows of a token, pairs of a row
 };
 
 template <int DT, bool VEC, bool INTER>
@@ -172,23 +210,41 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(const RotArgs a) {
   const int64_t all = (int64_t)a.batch * a.tokens;
   const int64_t n0 = (int64_t)blockIdx.x * a.per;
   const int nt = (int)(all - n0 < a.per ? all - n0 : a.per);
+  // the group's first token's batch element and place; the others follow
+  const int b0 = (int)(n0 / a.tokens), s0 = (int)(n0 - (int64_t)b0 * a.tokens);
+  auto place = [&](int t, int64_t& b, int64_t& s) {
+    b = b0, s = s0 + t;
+    while (s >= a.tokens) s -= a.tokens, ++b;
+  };
   for (int i = tid; i < nt * h; i += kRotThreads) {
-    const int t = i / h, f = i - t * h;
-    const int64_t b = (n0 + t) / a.tokens, s = (n0 + t) - b * a.tokens;
+    const int t = a.by_half(i), f = i - t * h;
+    int64_t b, s;
+    place(t, b, s);
     sc[t][f] = angle_of(position_at(a.positions, a.positions_64, b * a.pos_sb + s), a.inv_freq[f], a.scale, a.backward);
   }
   __syncthreads();
   const int nu = R::count(a.rot, a.d);
-  const int rows = a.heads[0] + a.heads[1];
-  for (int i = tid; i < nt * rows * nu; i += kRotThreads) {
-    const int r = i / nu, u = i - r * nu;
-    const int t = r / rows;
+  const int rows = a.heads[0] + a.heads[1], vecs = nt * rows * nu;
+  auto read = [&](int i, TurnVec<DT, VEC, INTER>& v) {
+    const int r = a.by_nu(i);
+    v.u = i - r * nu;
+    const int t = a.by_rows(r);
     int head = r - t * rows;
     const int w = head >= a.heads[0];
     if (w) head -= a.heads[0];
-    const int64_t b = (n0 + t) / a.tokens, s = (n0 + t) - b * a.tokens;
-    turn_vec<DT, VEC, INTER>(a.x[w] + b * a.x_sb[w] + head * a.x_sh[w] + s * a.x_ss[w],
-                             a.y[w] + b * a.y_sb[w] + head * a.y_sh[w] + s * a.y_ss[w], DT, R::ES, 1.f, u, a.rot, sc[t]);
+    int64_t b, s;
+    place(t, b, s);
+    v.dst = a.y[w] + b * a.y_sb[w] + head * a.y_sh[w] + s * a.y_ss[w];
+    v.sc = sc[t], v.div = 1.f, v.rot = a.rot, v.dtype = DT, v.es = R::ES;
+    v.read(a.x[w] + b * a.x_sb[w] + head * a.x_sh[w] + s * a.x_ss[w]);
+  };
+  for (int i = tid; i < vecs; i += 2 * kRotThreads) {
+    TurnVec<DT, VEC, INTER> v0, v1;
+    const bool two = i + kRotThreads < vecs;
+    read(i, v0);
+    if (two) read(i + kRotThreads, v1);
+    v0.finish();
+    if (two) v1.finish();
   }
 }
 
@@ -207,6 +263,7 @@ struct AppendArgs {
   const double* inv_freq;
   float scale, k_scale, v_scale;
   int32_t* error_flag;
+  Div by_nu, by_nc, by_per, by_half;  // vectors of a turned row, of a copied one, of a token; pairs of a row
 };
 
 // The sequence of row `row`: the last b with cu[b] <= row, -1 where cu[0] > row.
@@ -268,7 +325,7 @@ __global__ __launch_bounds__(kRotThreads) void append_kernel(const AppendArgs a)
   __syncthreads();
   const int h = a.rot / 2;
   for (int i = tid; i < nt * h; i += kRotThreads) {
-    const int t = i / h, f = i - t * h;
+    const int t = a.by_half(i), f = i - t * h;
     sc[t][f] = angle_of(pos[t], a.inv_freq[f], a.scale, false);
   }
   __syncthreads();
@@ -277,36 +334,50 @@ __global__ __launch_bounds__(kRotThreads) void append_kernel(const AppendArgs a)
   const int nq = a.Hq * nu, nk = a.Hkv * nu, nv = a.Hkv * nc;
   const int per = nq + nk + nv;
   const int es = a.cache_dtype == OC_F32 ? 4 : (a.cache_dtype == OC_FP8_E4M3FN ? 1 : 2);
-  for (int i = tid; i < nt * per; i += kRotThreads) {
-    const int t = i / per;
+  // vector i of the group's tokens; false where there is nothing to store
+  auto read = [&](int i, TurnVec<DT, VEC, INTER>& v) {
+    const int t = a.by_per(i);
     int j = i - t * per;
     const int64_t row = n0 + t;
     const int64_t id = blk[t];
+    v.sc = sc[t], v.rot = a.rot;
     if (j < nq) {
-      const int head = j / nu, u = j - head * nu;
-      char* o = a.q_out + row * a.o_ss + head * a.o_sh;
+      const int head = a.by_nu(j);
+      v.u = j - head * nu;
+      v.dst = a.q_out + row * a.o_ss + head * a.o_sh;
       if (id == -2) {  // no token: its queries are zeros
         const float z[1] = {0.f};
-        for (int c = u; c < a.d; c += nu) store_n<1>(o + c * R::ES, DT, 1.f, z);
-      } else {
-        turn_vec<DT, VEC, INTER>(a.q + row * a.q_ss + head * a.q_sh, o, DT, R::ES, 1.f, u, a.rot, sc[t]);
+        for (int c = v.u; c < a.d; c += nu) store_n<1>(v.dst + c * R::ES, DT, 1.f, z);
+        return false;
       }
-      continue;
+      v.div = 1.f, v.dtype = DT, v.es = R::ES;
+      v.read(a.q + row * a.q_ss + head * a.q_sh);
+      return true;
     }
+    if (id < 0) return false;
     j -= nq;
-    if (id < 0) continue;
+    v.dtype = a.cache_dtype, v.es = es;
     if (j < nk) {
-      const int head = j / nu, u = j - head * nu;
-      turn_vec<DT, VEC, INTER>(a.k + row * a.k_ss + head * a.k_sh,
-                               a.kc + id * a.kc_sb + head * a.kc_sh + slot[t] * a.kc_ss, a.cache_dtype, es, a.k_scale,
-                               u, a.rot, sc[t]);
+      const int head = a.by_nu(j);
+      v.u = j - head * nu, v.div = a.k_scale;
+      v.dst = a.kc + id * a.kc_sb + head * a.kc_sh + slot[t] * a.kc_ss;
+      v.read(a.k + row * a.k_ss + head * a.k_sh);
     } else {
       j -= nk;
-      const int head = j / nc, u = j - head * nc;
-      turn_vec<DT, VEC, INTER>(a.v + row * a.v_ss + head * a.v_sh,
-                               a.vc + id * a.vc_sb + head * a.vc_sh + slot[t] * a.vc_ss, a.cache_dtype, es, a.v_scale,
-                               u, 0, sc[t]);
+      const int head = a.by_nc(j);
+      v.u = j - head * nc, v.div = a.v_scale, v.rot = 0;
+      v.dst = a.vc + id * a.vc_sb + head * a.vc_sh + slot[t] * a.vc_ss;
+      v.read(a.v + row * a.v_ss + head * a.v_sh);
     }
+    return true;
+  };
+  const int all = nt * per;
+  for (int i = tid; i < all; i += 2 * kRotThreads) {
+    TurnVec<DT, VEC, INTER> v0, v1;
+    const bool one = read(i, v0);
+    const bool two = i + kRotThreads < all && read(i + kRotThreads, v1);
+    if (one) v0.finish();
+    if (two) v1.finish();
   }
 }
 
@@ -320,6 +391,12 @@ bool multiple(std::initializer_list<int64_t> v, int64_t of) {
 bool whole_vecs(int dtype, int d, int rot, bool inter) {
   const int n = dtype == OC_F32 ? 4 : 8;
   return (inter ? rot % n == 0 : (rot / 2) % n == 0) && (d - rot) % n == 0 && d % n == 0;
+}
+
+// RowVecs' numbers of vectors, for the host
+int row_vecs(int dtype, bool vec, bool inter, int rot, int d) {
+  const int n = vec ? (dtype == OC_F32 ? 4 : 8) : 1;
+  return (inter ? rot / (vec ? n : 2) : rot / 2 / n) + (d - rot) / n;
 }
 
 template <int DT, typename K1, typename K2, typename K3, typename K4, typename Args>
@@ -383,6 +460,8 @@ extern "C" int oc_apply_rotary(const oc_rotary_params* p, void* stream) {
   const int64_t blocks = (all + a.per - 1) / a.per;
   if (blocks > 0x7FFFFFFF) return fail(OC_ERR_UNSUPPORTED, "too many tokens");
   const bool inter = p->interleaved != 0;
+  a.by_nu = Div(std::max(row_vecs(p->dtype, vec, inter, a.rot, a.d), 1));
+  a.by_rows = Div(a.heads[0] + a.heads[1]), a.by_half = Div(std::max(a.rot / 2, 1));
   const hipStream_t s = (hipStream_t)stream;
   if (p->dtype == OC_F32) launch_rotary<OC_F32>(vec, inter, (unsigned)blocks, s, a);
   else if (p->dtype == OC_F16) launch_rotary<OC_F16>(vec, inter, (unsigned)blocks, s, a);
@@ -438,6 +517,9 @@ extern "C" int oc_append_paged(const oc_append_params* p, void* stream) {
   a.per = tokens_per_group(p->tokens);
   const unsigned blocks = (unsigned)((p->tokens + a.per - 1) / a.per);
   const bool inter = p->interleaved != 0;
+  const int nu = row_vecs(p->dtype, vec, inter, rot, a.d), nc = row_vecs(p->dtype, vec, inter, 0, a.d);
+  a.by_nu = Div(std::max(nu, 1)), a.by_nc = Div(nc), a.by_half = Div(std::max(rot / 2, 1));
+  a.by_per = Div(std::max((a.Hq + a.Hkv) * nu + a.Hkv * nc, 1));
   const hipStream_t s = (hipStream_t)stream;
   if (p->dtype == OC_F32) launch_append<OC_F32>(vec, inter, blocks, s, a);
   else if (p->dtype == OC_F16) launch_append<OC_F16>(vec, inter, blocks, s, a);
