@@ -80,60 +80,59 @@ struct Sight {
   const int* tdoc;           // LDS: documents of the tile's 64 tokens
 };
 
-// The cap: a raw score c becomes tanh(k c), k = scale / cap.  float32 takes
-// tanhf.  The 16-bit kernels take y times a cubic in y^2 while |y| = |k c| is at
-// most kTanhFit (tanh(y) / y, fitted with a relative error of 5.5e-7 there), and
-// 1 - 2 / (1 + e^2y) with the hardware's exponential and reciprocal where a
-// score of the wave's tile is larger: six full-rate instructions against three
-// and two quarter-rate ones.
-constexpr float kTanhFit = 0.5f;
-constexpr float kTanh0 = 0.999999456f, kTanh1 = -0.333263178f, kTanh2 = 0.131902954f, kTanh3 = -0.0444021952f;
+// What a head's scores go through: z = s (c - slope |i - j|) in base-2 units,
+// with c the raw score, or its tanh in the same units near zero (cap_scores),
+// and s = pre.  Where pre is negative or next to nothing, c is multiplied by it,
+// and s is 1.
+constexpr float kSmallest = 1e-6f;
+struct Change {
+  float s;
+  float pre;         // scale log2(e), times kTanh0 with a cap
+  float slope;       // the head's slope log2(e) / s
+  float k, inv;      // scale / cap, 1 / (kTanh0 k)
+  float lim, b1, b2; // |c| up to which the polynomial holds, its coefficients
+};
+
+// The cap: a raw score c becomes tanh(k c) / (kTanh0 k), k = scale / cap.
+// float32 takes tanhf.  The 16-bit kernels take c (1 + b1 c^2 + b2 c^4) while
+// |k c| is at most kTanhFit (tanh(y) / y by a quadratic in y^2, fitted with a
+// relative error of 4.0e-7 there), and 1 - 2 / (1 + e^2y) with the hardware's
+// exponential and reciprocal where a score of the wave's tile is larger: four
+// full-rate instructions against three and two quarter-rate ones.
+constexpr float kTanhFit = 0.25f;
+constexpr float kTanh0 = 0.999999604f, kTanh1 = -0.333219082f, kTanh2 = 0.128416128f;
 
 template <int DT>
-__device__ __forceinline__ void cap_scores(f32x4 (&c)[4], float k) {
+__device__ __forceinline__ void cap_scores(f32x4 (&c)[4], const Change& h) {
   if constexpr (DT == OC_F32) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[tb][i] = tanhf(c[tb][i] * k);
+      for (int i = 0; i < 4; ++i) c[tb][i] = tanhf(c[tb][i] * h.k) * h.inv;
   } else {
     float top = 0.f;
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[tb][i] *= k;
-        top = fmaxf(top, fabsf(c[tb][i]));
-      }
-    if (__builtin_amdgcn_ballot_w64(top > kTanhFit)) {
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(c[tb][i]));
+    if (__builtin_amdgcn_ballot_w64(top > h.lim)) {
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           c[tb][i] = __builtin_fmaf(
-              -2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(c[tb][i] * (2.f * kLog2e))), 1.f);
+              -2.f * h.inv, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(c[tb][i] * (2.f * kLog2e * h.k))), h.inv);
     } else {
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y = c[tb][i], u = y * y;
-          c[tb][i] = y * __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(kTanh3, u, kTanh2), u, kTanh1), u, kTanh0);
+          const float u = c[tb][i] * c[tb][i];
+          c[tb][i] *= __builtin_fmaf(__builtin_fmaf(h.b2, u, h.b1), u, 1.f);
         }
     }
   }
 }
-
-// What a head's scores go through: z = s (c - slope |i - j|) in base-2 units,
-// with c the raw score or its tanh, and s = pre.  Where pre is negative or next
-// to nothing, c is multiplied by it, and s is 1.
-constexpr float kSmallest = 1e-6f;
-struct Change {
-  float s;
-  float pre;    // cap log2(e) with a cap, else scale log2(e)
-  float k;      // scale / cap
-  float slope;  // the head's slope log2(e) / s
-};
 
 // Online-softmax update of one tile (as pf_softmax) with the scores changed: c
 // becomes 2^(z - m) for the tokens seen, 0 for the others.
@@ -141,7 +140,7 @@ template <int DT, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16], f32x4 (&c)[4], const Change& h,
                                                const Sight& e, int tok0, bool full) {
   float mt = -__builtin_inff();
-  if constexpr (CAP) cap_scores<DT>(c, h.k);
+  if constexpr (CAP) cap_scores<DT>(c, h);
   if (h.pre < kSmallest) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb) c[tb] *= h.pre;
@@ -462,10 +461,21 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   const char* kh = a.k + (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh;
   const char* vh = a.v + (int64_t)b * a.v_sb + (int64_t)kv * a.v_sh;
   Change change;
-  change.pre = (CAP ? a.cap : a.scale) * kLog2e;
+  change.pre = a.scale * kLog2e * (CAP ? kTanh0 : 1.f);
   change.s = change.pre < kSmallest ? 1.f : change.pre;
-  change.k = CAP ? a.scale / a.cap : 0.f;
   change.slope = BIAS ? a.slopes[h] * kLog2e / change.s : 0.f;
+  const auto same = [](float f) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f))); };
+  change.pre = same(change.pre);
+  change.s = same(change.s);
+  if (BIAS) change.slope = same(change.slope);
+  if constexpr (CAP) {
+    const float k = same(a.scale / a.cap), k2 = k * k;
+    change.k = k;
+    change.inv = same(k == 0.f ? 0.f : 1.f / (kTanh0 * k));  // (scale 0: every score is 0)
+    change.lim = same(k2 * k2 < 1e30f ? kTanhFit / fabsf(k) : -1.f);  // (k^4 has to be finite)
+    change.b1 = same(kTanh1 / kTanh0 * k2);
+    change.b2 = same(kTanh2 / kTanh0 * k2 * k2);
+  }
 
   // The tiles of the workgroup, 64 at a time, and what is true of each: that the
   // wave needs it, that all its queries see all of it (documents apart), that
