@@ -172,11 +172,12 @@ typedef struct oc_attend_prompt_params {
   const int32_t* documents;       /* (batch, kv_len) or NULL */
   int64_t documents_stride_b;
   oc_score_mods mods;
-  void* workspace;                /* oc_attend_prompt_workspace_size(p) bytes, any content */
+  void* workspace;                /* oc_attend_prompt_workspace_size(p) bytes, 16-byte aligned, any content */
   size_t workspace_bytes;
 } oc_attend_prompt_params;
 
-/* bytes of workspace oc_attend_prompt needs (0 without documents) */
+/* bytes of workspace oc_attend_prompt needs, from p's sizes, types, window and whether it has documents and prefix_lens
+   (0 for many calls without documents) */
 size_t oc_attend_prompt_workspace_size(const oc_attend_prompt_params* p);
 int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream);
 

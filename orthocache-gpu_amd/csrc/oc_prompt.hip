@@ -15,6 +15,7 @@
 // (prompt_pv_any).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -48,7 +49,22 @@ struct PromptArgs {
   float scale, cap;
   int32_t window;
   int32_t o_vec;  // out rows 8-byte aligned
+  // The tiles of a workgroup's queries in shares of share_tiles (0: one share).
+  // Each share's sums, of row ((b Hq + h) Sq + query) shares + share: m, l, acc.
+  int32_t shares, share_tiles;
+  float *pm, *pl, *pacc;
 };
+
+// The tiles that queries at places lo .. hi may see, as a range.
+struct TileRange {
+  int lo, hi;
+};
+__device__ __forceinline__ TileRange tile_range(int lo, int hi, int window, int prefix, int kv_len) {
+  return {prefix > 0 || window >= lo ? 0 : (lo - window + 1) / 64, (min(max(max(hi + 1, prefix), 0), kv_len) + 63) / 64};
+}
+__device__ __forceinline__ int prefix_of(const int32_t* prefix, int b, int kv_len) {
+  return prefix ? min(max(prefix[b], 0), kv_len) : 0;
+}
 
 // The kernel's arguments, read again from memory where they are used: held
 // across the tile loop they would fill the scalar registers and push others out.
@@ -423,7 +439,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   const int off = a.Skv - a.Sq;
   const int x = lane & 15;
   const int window = a.window > 0 ? a.window : INT_MAX;
-  const int prefix = a.prefix ? min(max(a.prefix[b], 0), a.Skv) : 0;
+  const int prefix = prefix_of(a.prefix, b, a.Skv);
   const int32_t* docs = a.docs ? a.docs + b * a.docs_sb : nullptr;
   auto doc_at = [&](int s) {  // the document of query s, -1 for none
     const int p = s + off;
@@ -451,7 +467,14 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
     return 64 * t + 63 < a.Skv &&
            ((64 * t + 63 <= lo && (window == INT_MAX || hi - 64 * t < window)) || 64 * t + 63 < prefix);
   };
-  const int t_hi = (min(max(max(g_hi + 1, prefix), 0), a.Skv) + 63) / 64;
+  const TileRange all = tile_range(g_lo, g_hi, window, prefix, a.Skv);
+  int t_hi = all.hi;
+  int t_lo = 0;
+  if (a.shares > 1) {
+    t_lo = all.lo + (int)blockIdx.y * a.share_tiles;
+    t_hi = min(t_hi, t_lo + a.share_tiles);
+    if (t_lo >= t_hi) return;  // nothing to see: the join counts on no such share
+  }
   const bool active = pos0 < a.Sq;
 
   PrefillArgs pa;  // what the tile staging and the q load read
@@ -465,9 +488,10 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   change.s = change.pre < kSmallest ? 1.f : change.pre;
   change.slope = BIAS ? a.slopes[h] * kLog2e / change.s : 0.f;
   const auto same = [](float f) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f))); };
-  change.pre = same(change.pre);
-  change.s = same(change.s);
-  if (BIAS) change.slope = same(change.slope);
+  if constexpr (CAP) {
+    change.pre = same(change.pre);
+    change.s = same(change.s);
+  }
   if constexpr (CAP) {
     const float k = same(a.scale / a.cap), k2 = k * k;
     change.k = k;
@@ -530,9 +554,10 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   // more registers than two workgroups a CU leave.)
   auto pass = [&](auto any_c) -> bool {
     constexpr bool ANY = decltype(any_c)::value;
-    word = 0;
+    word = t_lo / 64;
     bits = 0;
-    if (t_hi > 0) load_word(0);
+    if (t_lo < t_hi) load_word(word);
+    bits &= ~0ull << (t_lo & 63);
     st = PfState{kNoScore, 0.f, 0.f, 0};
 #pragma unroll
     for (int nc = 0; nc < D / 16; ++nc) accp[nc] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -641,7 +666,13 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   asm volatile("" : "+v"(tl));
   const int qpos = pos0 + (tl & 15), r = (tl >> 4) & 3;
   const auto ap = prompt_args();
-  if (qpos < ap->Sq) {
+  if (qpos >= ap->Sq) return;
+  if (ap->shares > 1) {
+    const int64_t row = (((int64_t)b * ap->Hq + h) * ap->Sq + qpos) * ap->shares + blockIdx.y;
+    if (r == 0) ap->pm[row] = st.m, ap->pl[row] = l;
+#pragma unroll
+    for (int nc = 0; nc < D / 16; ++nc) *reinterpret_cast<f32x4*>(ap->pacc + row * D + 16 * nc + 4 * r) = accp[nc];
+  } else {
     char* orow = ap->out + (int64_t)b * ap->o_sb + (int64_t)h * ap->o_sh + (int64_t)qpos * ap->o_ss;
 #pragma unroll
     for (int nc = 0; nc < D / 16; ++nc) {
@@ -664,12 +695,56 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   }
 }
 
+// Joins the shares of a query: out = sum w acc / sum w l with w = 2^(m - max m).
+// D / 4 threads a query; a share in which it sees nothing has l = 0, and the
+// shares behind its workgroup's last tile were not run.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs a) {
+  constexpr int LANES = D / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (row >= (int64_t)a.B * a.Hq * a.Sq) return;
+  const int col = 4 * (threadIdx.x % LANES);
+  const int q = (int)(row % a.Sq), bh = (int)(row / a.Sq), b = bh / a.Hq, h = bh % a.Hq;
+  const int first = q / kPfRows * kPfRows, off = a.Skv - a.Sq;
+  const TileRange t = tile_range(first + off, min(first + kPfRows, a.Sq) - 1 + off, a.window > 0 ? a.window : INT_MAX,
+                                 prefix_of(a.prefix, b, a.Skv), a.Skv);
+  const int n = (max(t.hi - t.lo, 0) + a.share_tiles - 1) / a.share_tiles;
+  const int64_t r = row * a.shares;
+  float M = kNoScore, l = 0.f;
+  for (int s = 0; s < n; ++s) M = fmaxf(M, a.pm[r + s]);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n; ++s) {
+    const float w = __builtin_amdgcn_exp2f(a.pm[r + s] - M), ls = a.pl[r + s];
+    if (ls == 0.f || (w == 0.f && ls == ls)) continue;  // (0 times an infinite sum; a NaN stays one)
+    l += w * ls;
+    x += w * *reinterpret_cast<const f32x4*>(a.pacc + (r + s) * D + col);
+  }
+  x *= l == 0.f ? 0.f : 1.f / l;
+  char* o = a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)q * a.o_ss;
+  if constexpr (DT == OC_F32) {
+    *reinterpret_cast<f32x4*>(o + 4 * col) = x;
+  } else {
+    const uint2 w = {pf_pack<DT>(x[0], x[1]), pf_pack<DT>(x[2], x[3])};
+    uint16_t* o16 = reinterpret_cast<uint16_t*>(o) + col;
+    if (a.o_vec) {
+      *reinterpret_cast<uint2*>(o16) = w;
+    } else {
+      o16[0] = (uint16_t)w.x, o16[1] = (uint16_t)(w.x >> 16);
+      o16[2] = (uint16_t)w.y, o16[3] = (uint16_t)(w.y >> 16);
+    }
+  }
+}
+
 template <int DT, int D>
 void launch_prompt(const PromptArgs& a, unsigned blocks, hipStream_t s) {
   const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
   auto k = cap ? (bias ? prompt_kernel<DT, D, true, true> : prompt_kernel<DT, D, true, false>)
                : (bias ? prompt_kernel<DT, D, false, true> : prompt_kernel<DT, D, false, false>);
-  hipLaunchKernelGGL(k, dim3(blocks), dim3(kPfThreads), 0, s, a);
+  hipLaunchKernelGGL(k, dim3(blocks, (unsigned)a.shares), dim3(kPfThreads), 0, s, a);
+  if (a.shares > 1) {
+    const int64_t rows = (int64_t)a.B * a.Hq * a.Sq, per = 256 / (D / 4);
+    hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a);
+  }
 }
 
 template <int DT>
@@ -692,14 +767,55 @@ int check_prompt(const oc_attend_prompt_params* p) {
   return check_mods(&p->mods);
 }
 
+// With few queries the CUs stand idle while one workgroup after the other goes
+// through a long context alone: the tiles are then split over several, and
+// prompt_join_kernel adds up their sums.  The shares would fill every CU with
+// the workgroups it holds, and are of eight tiles or more (float32, whose tiles
+// take longer: four).  Each costs its sums, written and read, and the join a
+// launch, so a call is split where by these times (of a tile, in ns; two
+// workgroups on one CU take 0.9 of twice as long) it ends sooner.  Measured on
+// 256 CUs, one pass against shares, bf16 / f16, head_dim 128: 16 queries on
+// 32768 tokens (32 heads) 577 and 62 us, 128 on 4096 103 and 36, 512 on 4096
+// 101 and 62, 8 heads of 1024 / 2048 / 4096 tokens 30 and 25, 52 and 41, 98
+// and 80; float32, 4 heads of 1341 tokens, 183 and 57.  Not split by the rule:
+// 32 heads of 1024 (29, shares 39) and 24 of 2560 (69, shares 83).
+struct Shares {
+  int tiles, n;  // tiles of each, and how many
+};
+Shares prompt_shares(const oc_attend_prompt_params* p) {
+  const bool f32 = p->dtype == OC_F32, wide = p->head_dim == 128;
+  const int64_t all = (p->kv_len + 63) / 64, blocks = (int64_t)p->batch * p->num_q_heads * ((p->q_len + kPfRows - 1) / kPfRows);
+  // the most tiles that a workgroup sees, and those of one in the middle
+  const int64_t most = p->mods.window > 0 && !p->mods.prefix_lens
+                           ? std::min<int64_t>(all, ((int64_t)p->mods.window + kPfRows + 63) / 64 + 1) : all;
+  const int64_t mean = std::min<int64_t>(most, std::max<int64_t>(1, (p->kv_len - p->q_len / 2 + 64) / 64));
+  const int64_t cus = device_cus(), room = f32 && wide ? cus : 2 * cus;
+  const int64_t tiles = std::max<int64_t>(f32 ? 4 : 8, (blocks * mean + room - 1) / room);
+  if (blocks >= 2 * cus || 2 * most < 3 * tiles) return {0, 1};
+  const double tile_ns = f32 ? (wide ? 9000 : 5000) : (wide ? 1500 : 1150);
+  const double busy = 0.9 * blocks * mean / cus;  // tiles of a CU, if all had the same
+  const double one = tile_ns * std::max<double>(most, busy);
+  const double sums = (blocks * mean / (double)tiles + blocks / 2.) * kPfRows * p->head_dim * 8;
+  const double split = tile_ns * std::max<double>(tiles, busy) + sums / 4900 + 4500;
+  return split < one ? Shares{(int)tiles, (int)((most + tiles - 1) / tiles)} : Shares{0, 1};
+}
+
+// bytes of the documents' ranges, in the workspace before the shares' sums (which begin at a multiple of 16)
+size_t range_bytes(const oc_attend_prompt_params* p) {
+  return p->documents ? (size_t)p->batch * (size_t)((p->kv_len + 63) / 64) * sizeof(int2) : 0;
+}
+
 }  // namespace
 }  // namespace oc
 
 using namespace oc;
 
 extern "C" size_t oc_attend_prompt_workspace_size(const oc_attend_prompt_params* p) {
-  if (check_prompt(p) != OC_OK || !p->documents) return 0;
-  return (size_t)p->batch * (size_t)((p->kv_len + 63) / 64) * sizeof(int2);
+  if (check_prompt(p) != OC_OK) return 0;
+  const Shares n = prompt_shares(p);
+  if (n.n == 1) return range_bytes(p);
+  const size_t rows = (size_t)p->batch * p->num_q_heads * p->q_len * n.n;
+  return (range_bytes(p) + 15) / 16 * 16 + (rows + 3) / 4 * 4 * 8 + rows * p->head_dim * 4;
 }
 
 extern "C" int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream) {
@@ -722,6 +838,7 @@ extern "C" int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream) 
   const size_t need = oc_attend_prompt_workspace_size(p);
   if (need && (!p->workspace || p->workspace_bytes < need))
     return fail(OC_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", p->workspace_bytes, need);
+  if (need && (uintptr_t)p->workspace % 16) return fail(OC_ERR_INVALID, "the workspace must be 16-byte aligned");
   PromptArgs a{};
   a.q = (const char*)p->q, a.k = (const char*)p->k, a.v = (const char*)p->v, a.out = (char*)p->out;
   a.q_sb = p->q_stride_b * es, a.q_sh = p->q_stride_h * es, a.q_ss = p->q_stride_s * es;
@@ -736,6 +853,10 @@ extern "C" int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream) 
   a.slopes = p->mods.slopes, a.prefix = p->mods.prefix_lens;
   a.evict = a.T > 0 ? p->mods.evict : nullptr, a.e_sb = p->mods.evict_stride_b, a.e_sh = p->mods.evict_stride_h;
   a.scale = p->mods.scale, a.cap = p->mods.softcap, a.window = p->mods.window;
+  const Shares shares = prompt_shares(p);
+  a.shares = shares.n, a.share_tiles = shares.tiles;
+  const size_t rows = ((size_t)p->batch * p->num_q_heads * p->q_len * shares.n + 3) / 4 * 4;
+  a.pm = (float*)((char*)p->workspace + (range_bytes(p) + 15) / 16 * 16), a.pl = a.pm + rows, a.pacc = a.pl + rows;
   const int64_t blocks = (int64_t)p->batch * p->num_q_heads * a.qblocks;
   const int64_t tiles = (int64_t)p->batch * ((p->kv_len + 63) / 64);
   if (blocks > 0x7FFFFFFF || tiles > 0x7FFFFFFF || (int64_t)p->batch * p->num_q_heads > 0x7FFFFFFF)

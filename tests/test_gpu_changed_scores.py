@@ -399,6 +399,79 @@ def test_prompt_unseen_values_have_no_effect(dt, d):
         _check_prompt(B, q, k3, v2, what=str(kw), **check)
 
 
+SHARES = [dict(), dict(softcap=20.0, slopes=True), dict(window=700), dict(window=70, prefix=True), dict(docs=5), dict(evict=0.5, docs=-1)]
+
+
+@pytest.mark.parametrize("change", range(len(SHARES)))
+@pytest.mark.parametrize("sq,skv", [(1, 4097), (130, 2000), (1341, 1341), (1500, 1400)])
+@pytest.mark.parametrize("dt,d", [(torch.float32, 64), (torch.float32, 128), (torch.float16, 128), (torch.bfloat16, 64)], ids=str)
+def test_prompt_shares(dt, d, sq, skv, change):
+    """Few queries on a long context: tiles in shares, some of which see nothing, some rows nothing at all."""
+    import orthocache_gpu as oc
+    c = dict(SHARES[change])
+    B, hq, hkv = 2, 2, 1
+    q, k, v = _randn((B, hq, sq, d), dt, 1), _randn((B, hkv, skv, d), dt, 2), _randn((B, hkv, skv, d), dt, 3)
+    slopes = _slopes(hq) if c.pop("slopes", False) else None
+    prefix = torch.tensor([900, 0], dtype=torch.int32, device=DEV) if c.pop("prefix", False) else None
+    docs, evict = c.pop("docs", None), c.pop("evict", None)
+    g = torch.Generator().manual_seed(skv + change)
+    if docs is not None:
+        docs = torch.randint(-1, 2, (B, skv), generator=g) if docs < 0 else torch.sort(torch.randint(0, docs, (B, skv), generator=g), 1).values
+        docs = docs.to(torch.int32).to(DEV)
+    if evict is not None:
+        evict = torch.rand((B, hkv, skv // 64), generator=g) < evict
+        evict[0] = True  # nothing but the last tile, where it is not a whole one
+        evict = evict.to(DEV)
+    out = oc.attend_prompt(q, k, v, alibi_slopes=slopes, prefix_lens=prefix, documents=docs, evict_mask=evict, **c)
+    _check_prompt(out, q, k, v, slopes=slopes, prefix=prefix, docs=docs, evict=evict, **c)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+def test_prompt_shares_not_finite(dt):
+    """A NaN in one share makes its rows NaN, an infinite V shows in its column, and what is not seen has no effect."""
+    import orthocache_gpu as oc
+    n, m, d = 20, 3000, 128
+    q, k, v = _randn((1, 2, n, d), dt, 1), _randn((1, 1, m, d), dt, 2), _randn((1, 1, m, d), dt, 3)
+    docs = torch.zeros(m, dtype=torch.int32, device=DEV)
+    docs[500:900] = -1
+    want = oc.attend_prompt(q, k, v, documents=docs)
+    _check_prompt(want, q, k, v, docs=docs)
+    k2, v2 = k.clone(), v.clone()
+    k2[:, :, 500:900], v2[:, :, 500:900] = NAN, INF
+    assert torch.equal(oc.attend_prompt(q, k2, v2, documents=docs), want)
+    k3 = k2.clone()
+    k3[0, 0, m - 5] = NAN  # seen by the last five queries, in the last share
+    got = oc.attend_prompt(q, k3, v2, documents=docs)
+    assert bool(torch.isnan(got[:, :, -5:]).all()) and torch.equal(got[:, :, :-5], want[:, :, :-5])
+    k3 = k2.clone()
+    k3[0, 0, 70] = NAN  # by all, in the first
+    assert bool(torch.isnan(oc.attend_prompt(q, k3, v2, documents=docs)).all())
+
+
+def test_prompt_shares_in_two_graphs():
+    """Two captured calls with shares, replayed at once: each has a workspace of its own."""
+    import orthocache_gpu as oc
+    sets = [tuple(_randn((1, h, n, 128), torch.float16, s + i) for i, (h, n) in enumerate(((4, 40), (2, 2500), (2, 2500)))) for s in (1, 9)]
+    want = [oc.attend_prompt(*x, softcap=3.0) for x in sets]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for x in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(oc.attend_prompt(*x, softcap=3.0))
+        graphs.append(g)
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        oc.attend_prompt(*sets[0])
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+
+
 def test_prompt_large_bias():
     """Scores far below zero, past -1e9: the nearest key that is left wins."""
     import orthocache_gpu as oc
