@@ -138,7 +138,7 @@ typedef struct oc_attend_paged_params {
   int32_t num_seqs, num_q_heads, num_kv_heads, head_dim;  /* head_dim a multiple of 8 up to 512 */
   float k_scale, v_scale;
   oc_score_mods mods;
-  int32_t num_splits;             /* parts of a sequence's tiles; 0: chosen from the sizes */
+  int32_t num_splits;             /* parts of a sequence's tiles (1024 at most); 0: chosen from the sizes */
   int32_t portable;               /* 1: the portable kernel whatever the shape */
   void* out;                      /* (num_seqs, num_q_heads, head_dim) */
   int64_t out_stride_b, out_stride_h;

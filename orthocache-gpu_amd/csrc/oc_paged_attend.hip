@@ -69,23 +69,61 @@ __device__ __forceinline__ float changed(const PagedArgs& a, float dot, float sl
   return __builtin_fmaf(-slope2, (float)dist, z * kLog2e);
 }
 
+// W words from p, aligned to all of them up to 16 bytes
+template <int W>
+__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+  if constexpr (W % 4 == 0) {
+#pragma unroll
+    for (int u = 0; u < W; u += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * u);
+      w[u] = x.x, w[u + 1] = x.y, w[u + 2] = x.z, w[u + 3] = x.w;
+    }
+  } else if constexpr (W == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    static_assert(W == 1);
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// the value of lane 4 (lane / 4) + I
+template <int I>
+__device__ __forceinline__ int64_t quad_lane(int64_t v) {
+  const int lo = __builtin_amdgcn_mov_dpp((int)v, 0x55 * I, 0xF, 0xF, true);
+  const int hi = __builtin_amdgcn_mov_dpp((int)(v >> 32), 0x55 * I, 0xF, 0xF, true);
+  return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+// the sum over the four lanes of a quad, in each of them
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));  // lanes 1 0 3 2
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
+}
+
 constexpr int kPortWaves = 4;
 constexpr int kPortThreads = kPortWaves * kWave;
 constexpr int kPortHeads = 4;  // query heads of a workgroup
 
 // The portable kernel: every head_dim (a multiple of 8 up to 512), block size
-// and type.  A wave takes a tile: a lane per token forms the scores of four
-// query heads, and then a lane per column adds up p.V token by token.
-template <int CT>
+// and type, four query heads a workgroup.  A wave takes a tile of 64 tokens.
+// Scores: a quad of lanes per token, eight columns each of 32, in four rounds
+// (a lane per token would read 64 rows at once, more than the L1 holds); then
+// lane i has the scores of token i.  p.V: the tokens seen are put together in
+// LDS, and a lane adds up four columns (twice four above head_dim 256) of every
+// TP-th of them, TP as many rows as 64 lanes hold, VA rows of loads ahead.
+template <int CT, int NI>
 __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const PagedArgs a) {
   constexpr int ES = Elem<CT>::size;
-  constexpr int NI = kPaMaxDim / kWave;
-  __shared__ float sq[kPortHeads][kPaMaxDim];
-  __shared__ float sp[kPortWaves][kPortHeads][kWave];
+  constexpr int VW = ES;  // words of four values
+  constexpr int DM = 256 * NI;
+  constexpr int VA = NI == 1 ? 8 : 4;  // steps of loads ahead
+  __shared__ __attribute__((aligned(16))) float sq[DM / 8 * 9][kPortHeads];
+  __shared__ __attribute__((aligned(16))) float sp[kPortWaves][kWave][kPortHeads];
   __shared__ int64_t srow[kPortWaves][kWave];
-  __shared__ float sacc[kPortHeads][kPaMaxDim];
+  __shared__ float sacc[kPortHeads][DM];
   __shared__ float sm[kPortWaves][kPortHeads], sl[kPortWaves][kPortHeads];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunks = (a.G + kPortHeads - 1) / kPortHeads;
   const int b = blockIdx.z, kv = blockIdx.y / chunks, split = blockIdx.x;
   const int g0 = (blockIdx.y % chunks) * kPortHeads;
@@ -93,21 +131,30 @@ __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const Page
   const int h0 = kv * a.G + g0;
   const Seen s = seen_of(a, b);
   const int qes = a.dtype == OC_F32 ? 4 : 2;
-  for (int i = tid; i < ng * a.d; i += kPortThreads) {
-    const int g = i / a.d, c = i - g * a.d;
-    sq[g][c] = load_scalar(a.q + b * a.q_sb + (h0 + g) * a.q_sh + c * qes, a.dtype);
+  // column c at row c + c / 8: the four lanes of a quad read in different banks; zeros up to a multiple of 32
+  auto q_row = [](int c) { return c + (c >> 3); };
+  const int dq = (a.d + 31) & ~31;
+  for (int i = tid; i < kPortHeads * dq; i += kPortThreads) {
+    const int g = i / dq, c = i - g * dq;
+    sq[q_row(c)][g] = g < ng && c < a.d ? load_scalar(a.q + b * a.q_sb + (h0 + g) * a.q_sh + c * qes, a.dtype) : 0.f;
   }
   __syncthreads();
   const int32_t* row = a.tables + b * a.bt_stride;
   const uint8_t* ev = a.evict ? a.evict + b * a.e_sb + kv * a.e_sh : nullptr;
-  float m[kPortHeads], l[kPortHeads], acc[kPortHeads][NI], slope2[kPortHeads];
+  // lanes of a V row (a power of two), and the lane's row and first column
+  const int lpr = min(64, 1 << (32 - __builtin_clz((a.d + 3) / 4 - 1)));
+  const int tp = 64 / lpr, mine = lane / lpr, col = 4 * (lane % lpr);
+  const int part = 8 * (lane & 3);
+  float m[kPortHeads], l[kPortHeads], acc[kPortHeads][NI][4], slope2[kPortHeads];
 #pragma unroll
   for (int g = 0; g < kPortHeads; ++g) {
     m[g] = kNoScore;
     l[g] = 0.f;
     slope2[g] = a.slopes && g < ng ? a.slopes[h0 + g] * kLog2e : 0.f;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) acc[g][i] = 0.f;
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[g][i][e] = 0.f;
   }
   const int64_t all = s.count();
   const int lo = (int)(all * split / a.P), hi = (int)(all * (split + 1) / a.P);
@@ -125,69 +172,111 @@ __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const Page
       }
     }
     const int slot = j & ((1 << a.block_log2) - 1);
-    float dot[kPortHeads] = {0.f, 0.f, 0.f, 0.f};
-    if (ok) {
-      const char* kp = a.k + id * a.k_sb + kv * a.k_sh + slot * a.k_ss;
-      for (int c = 0; c < a.d; c += 8) {
-        uint32_t w[2 * ES];
-        if constexpr (ES == 1) {
-          const uint2 u = *reinterpret_cast<const uint2*>(kp + c);
-          w[0] = u.x, w[1] = u.y;
-        } else {
+    const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
+    if (!seen) continue;
+    // K of token 4 quad + f in round f; of the tile's first token seen for those that are not
+    int64_t ko = id * a.k_sb + slot * a.k_ss;
+    const int one = __builtin_ctzll(seen);
+    const int64_t ko1 = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(ko >> 32), one) << 32) |
+                                  (uint32_t)__builtin_amdgcn_readlane((int)ko, one));
+    if (!ok) ko = ko1;
+    const char* kh = a.k + kv * a.k_sh;
+    const char* kp[4] = {kh + quad_lane<0>(ko), kh + quad_lane<1>(ko), kh + quad_lane<2>(ko), kh + quad_lane<3>(ko)};
+    float dots[4][kPortHeads] = {};
+    uint32_t w[4][2 * ES];
 #pragma unroll
-          for (int u = 0; u < ES / 2; ++u) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kp + c * ES + 16 * u);
-            w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
-          }
+    for (int f = 0; f < 4; ++f) load_words<2 * ES>(kp[f] + min(part, a.d - 8) * ES, w[f]);
+    for (int c0 = 0; c0 < a.d; c0 += 32) {
+      const int c = c0 + part;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        if (c0 + 32 > a.d && c >= a.d) {
+#pragma unroll
+          for (int u = 0; u < 2 * ES; ++u) w[f][u] = 0;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float kf = elem<CT>(w, e);
-#pragma unroll
-          for (int g = 0; g < kPortHeads; ++g) dot[g] = __builtin_fmaf(sq[g][c + e], kf, dot[g]);
+          const float kf = elem<CT>(w[f], e);
+          const float4 qv = *reinterpret_cast<const float4*>(sq[q_row(c) + e]);
+          dots[f][0] = __builtin_fmaf(qv.x, kf, dots[f][0]);
+          dots[f][1] = __builtin_fmaf(qv.y, kf, dots[f][1]);
+          dots[f][2] = __builtin_fmaf(qv.z, kf, dots[f][2]);
+          dots[f][3] = __builtin_fmaf(qv.w, kf, dots[f][3]);
         }
+        load_words<2 * ES>(kp[f] + min(c + 32, a.d - 8) * ES, w[f]);  // (the last again rather than a branch)
       }
     }
-    srow[wave][lane] = id * a.v_sb + slot * a.v_ss;
-    uint64_t left = __builtin_amdgcn_ballot_w64(ok);
+    float dot[kPortHeads];
 #pragma unroll
     for (int g = 0; g < kPortHeads; ++g) {
-      float z = g < ng && ok ? changed(a, dot[g], slope2[g], dist) : -__builtin_inff();
+#pragma unroll
+      for (int f = 0; f < 4; ++f) dots[f][g] = quad_sum(dots[f][g]);
+      dot[g] = lane & 2 ? (lane & 1 ? dots[3][g] : dots[2][g]) : (lane & 1 ? dots[1][g] : dots[0][g]);
+    }
+    float p[kPortHeads];
+#pragma unroll
+    for (int g = 0; g < kPortHeads; ++g) {
+      const float z = g < ng && ok ? changed(a, dot[g], slope2[g], dist) : -__builtin_inff();
       const float mt = fmaxf(m[g], wave_max(z));
       const float alpha = __builtin_amdgcn_exp2f(m[g] - mt);
-      const float p = __builtin_amdgcn_exp2f(z - mt);
-      l[g] = l[g] * alpha + wave_sum(p);
+      p[g] = __builtin_amdgcn_exp2f(z - mt);
+      l[g] = l[g] * alpha + wave_sum(p[g]);
       m[g] = mt;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) acc[g][i] *= alpha;
-      sp[wave][g][lane] = p;
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[g][i][e] *= alpha;
+    }
+    if (ok) {
+      const int u = __builtin_popcountll(seen & ((1ull << lane) - 1));
+      srow[wave][u] = id * a.v_sb + slot * a.v_ss;
+      *reinterpret_cast<float4*>(sp[wave][u]) = float4{p[0], p[1], p[2], p[3]};
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    while (left) {
-      const int u = __builtin_ctzll(left);
-      left &= left - 1;
-      const char* vp = a.v + kv * a.v_sh + srow[wave][u];
+    const char* vh = a.v + kv * a.v_sh + col * ES;
+    const int count = __builtin_popcountll(seen);
+    for (int u0 = mine; u0 < count + mine; u0 += VA * tp) {  // (uniform: a lane's rows are u0, u0 + tp, ..)
+      uint32_t w[VA][NI][VW];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = lane + 64 * i;
-        if (c < a.d) {
-          float vf;
-          if constexpr (CT == OC_FP8_E4M3FN) {
-            const uint32_t w[1] = {*reinterpret_cast<const uint8_t*>(vp + c)};
-            vf = elem<CT>(w, 0);
-          } else {
-            vf = load_scalar(vp + c * ES, CT);
-          }
+      for (int f = 0; f < VA; ++f) {
+        const int u = u0 + f * tp;
+        const bool in = u < count;
+        const char* vp = vh + srow[wave][in ? u : 0];
 #pragma unroll
-          for (int g = 0; g < kPortHeads; ++g) acc[g][i] = __builtin_fmaf(sp[wave][g][u], vf, acc[g][i]);
+        for (int i = 0; i < NI; ++i) {
+#pragma unroll
+          for (int e = 0; e < VW; ++e) w[f][i][e] = 0;
+          if (in && col + 256 * i < a.d) load_words<VW>(vp + 256 * i * ES, w[f][i]);
         }
+      }
+#pragma unroll
+      for (int f = 0; f < VA; ++f) {
+        const int u = u0 + f * tp;
+        const float4 pv = *reinterpret_cast<const float4*>(sp[wave][u < count ? u : 0]);  // (past the last: times 0)
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float vf = elem<CT>(w[f][i], e);
+            acc[0][i][e] = __builtin_fmaf(pv.x, vf, acc[0][i][e]);
+            acc[1][i][e] = __builtin_fmaf(pv.y, vf, acc[1][i][e]);
+            acc[2][i][e] = __builtin_fmaf(pv.z, vf, acc[2][i][e]);
+            acc[3][i][e] = __builtin_fmaf(pv.w, vf, acc[3][i][e]);
+          }
       }
     }
     __builtin_amdgcn_wave_barrier();
   }
-  // join the waves, in their order
+  // join the wave's rows, then the waves, in their order
+  for (int o = lpr; o < 64; o <<= 1)
+#pragma unroll
+    for (int g = 0; g < kPortHeads; ++g)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[g][i][e] += __shfl_xor(acc[g][i][e], o, 64);
 #pragma unroll
   for (int g = 0; g < kPortHeads; ++g)
     if (lane == 0) {
@@ -204,15 +293,17 @@ __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const Page
     for (int w = 0; w < kPortWaves; ++w) L[g] += sl[w][g] * __builtin_amdgcn_exp2f(sm[w][g] - M[g]);
   }
   for (int w = 0; w < kPortWaves; ++w) {
-    if (wave == w) {
+    if (wave == w && mine == 0) {
 #pragma unroll
       for (int g = 0; g < kPortHeads; ++g) {
         const float f = __builtin_amdgcn_exp2f(m[g] - M[g]);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int c = lane + 64 * i;
-          if (c < a.d) sacc[g][c] = (w ? sacc[g][c] : 0.f) + acc[g][i] * f;
-        }
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = col + 256 * i + e;
+            if (c < a.d) sacc[g][c] = (w ? sacc[g][c] : 0.f) + acc[g][i][e] * f;
+          }
       }
     }
     __syncthreads();
@@ -573,19 +664,61 @@ __global__ __launch_bounds__(kPmThreads) __attribute__((amdgpu_waves_per_eu(D ==
 }
 
 // Joins the shares of one (sequence, query head): out = sum w acc / sum w l
-// with w = 2^(m - max m).
+// with w = 2^(m - max m).  The weights are formed by all threads at once, then
+// each group of d / 4 threads adds up every so manieth share, four loads at a
+// time: one share after the other waits for memory as often as there are shares.
+constexpr int kMaxSplits = 1024;
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  __shared__ float sw[kMaxSplits], sm[4], sl[4];
+  __shared__ float4 sx[256];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = ((int64_t)b * a.Hq + h) * a.P;
   float M = kNoScore, L = 0.f;
-  for (int s = 0; s < a.P; ++s) M = fmaxf(M, a.pm[r + s]);
-  for (int s = 0; s < a.P; ++s) L += a.pl[r + s] * __builtin_amdgcn_exp2f(a.pm[r + s] - M);
-  const int es = a.dtype == OC_F32 ? 4 : 2;
-  for (int c = tid; c < a.d; c += 256) {
-    float x = 0.f;
-    for (int s = 0; s < a.P; ++s) x += a.pacc[(r + s) * a.d + c] * __builtin_amdgcn_exp2f(a.pm[r + s] - M);
-    store_scalar(a.out + b * a.o_sb + h * a.o_sh + c * es, a.dtype, L == 0.f ? 0.f : x * a.v_scale / L);
+  for (int s = tid; s < a.P; s += 256) M = fmaxf(M, a.pm[r + s]);
+  M = wave_max(M);
+  if (lane == 0) sm[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  for (int s = tid; s < a.P; s += 256) {
+    const float w = __builtin_amdgcn_exp2f(a.pm[r + s] - M), l = a.pl[r + s];
+    sw[s] = w;
+    if (w != 0.f || l != l) L += l * w;  // (a NaN stays one)
   }
+  L = wave_sum(L);
+  if (lane == 0) sl[wave] = L;
+  __syncthreads();
+  L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const int lanes = a.d / 4, groups = 256 / lanes, g = tid / lanes, c = 4 * (tid % lanes);
+  float4 x = {0.f, 0.f, 0.f, 0.f};
+  if (g < groups) {
+    auto add = [&](float w, const float4& v) {
+      if (w == 0.f) return;  // (0 times an infinite sum)
+      x.x += w * v.x, x.y += w * v.y, x.z += w * v.z, x.w += w * v.w;
+    };
+    const float* p = a.pacc + r * a.d + c;
+    int s = g;
+    for (; s + 3 * groups < a.P; s += 4 * groups) {
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const float4*>(p + (int64_t)(s + u * groups) * a.d);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) add(sw[s + u * groups], v[u]);
+    }
+    for (; s < a.P; s += groups) add(sw[s], *reinterpret_cast<const float4*>(p + (int64_t)s * a.d));
+    sx[tid] = x;
+  }
+  __syncthreads();
+  if (g > 0) return;
+  for (int u = 1; u < groups; ++u) {
+    const float4 v = sx[u * lanes + tid];
+    x.x += v.x, x.y += v.y, x.z += v.z, x.w += v.w;
+  }
+  const int es = a.dtype == OC_F32 ? 4 : 2;
+  const float f = L == 0.f ? 0.f : a.v_scale / L;
+  char* o = a.out + b * a.o_sb + h * a.o_sh + c * es;
+  const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) store_scalar(o + e * es, a.dtype, L == 0.f ? 0.f : y[e] * f);
 }
 
 int check_paged(const oc_attend_paged_params* p) {
@@ -623,11 +756,17 @@ bool paged_tuned(const oc_attend_paged_params* p) {
 // Shares of a sequence: about four workgroups per CU, at least four tiles each.
 int paged_splits(const oc_attend_paged_params* p) {
   const int64_t tiles = ((int64_t)p->max_blocks * p->block_size + 63) / 64;
-  if (p->num_splits > 0) return (int)std::max<int64_t>(1, std::min<int64_t>(p->num_splits, tiles));
+  if (p->num_splits > 0) return (int)std::max<int64_t>(1, std::min<int64_t>({p->num_splits, tiles, kMaxSplits}));
   const int64_t g = p->num_q_heads / p->num_kv_heads;
   const int heads = paged_tuned(p) ? kPmHeads : kPortHeads;
   const int64_t blocks = (int64_t)p->num_seqs * p->num_kv_heads * ((g + heads - 1) / heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({4 * (int64_t)device_cus() / std::max<int64_t>(blocks, 1), tiles / 4, 1024}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({4 * (int64_t)device_cus() / std::max<int64_t>(blocks, 1), tiles / 4, kMaxSplits}));
+}
+
+template <int CT>
+void launch_portable(const PagedArgs& a, dim3 grid, hipStream_t s) {
+  if (a.d <= 256) hipLaunchKernelGGL((paged_portable_kernel<CT, 1>), grid, dim3(kPortThreads), 0, s, a);
+  else hipLaunchKernelGGL((paged_portable_kernel<CT, 2>), grid, dim3(kPortThreads), 0, s, a);
 }
 
 template <int CT, int MT>
@@ -645,7 +784,8 @@ using namespace oc;
 extern "C" size_t oc_attend_paged_workspace_size(const oc_attend_paged_params* p) {
   if (check_paged(p) != OC_OK || p->num_q_heads == 0 || p->num_seqs == 0) return 0;
   const int P = paged_splits(p);
-  return P == 1 ? 0 : (size_t)p->num_seqs * p->num_q_heads * P * (p->head_dim + 2) * 4;
+  const size_t states = (size_t)p->num_seqs * p->num_q_heads * P;
+  return P == 1 ? 0 : (states + 3) / 4 * 4 * 8 + states * p->head_dim * 4;
 }
 
 extern "C" int oc_attend_paged(const oc_attend_paged_params* p, void* stream) {
@@ -675,7 +815,7 @@ extern "C" int oc_attend_paged(const oc_attend_paged_params* p, void* stream) {
   a.scale = p->mods.scale * p->k_scale, a.cap = p->mods.softcap, a.v_scale = p->v_scale;
   a.P = paged_splits(p), a.error_flag = p->error_flag;
   const int64_t rows = (int64_t)a.n * a.Hq;
-  a.pm = (float*)p->workspace, a.pl = a.pm + rows * a.P, a.pacc = a.pl + rows * a.P;
+  a.pm = (float*)p->workspace, a.pl = a.pm + (rows * a.P + 3) / 4 * 4, a.pacc = a.pl + (rows * a.P + 3) / 4 * 4;
   const hipStream_t s = (hipStream_t)stream;
   const bool tuned = paged_tuned(p);
   const int heads = tuned ? kPmHeads : kPortHeads;
@@ -687,10 +827,10 @@ extern "C" int oc_attend_paged(const oc_attend_paged_params* p, void* stream) {
     else if (p->dtype == OC_BF16) launch_paged_mfma<OC_FP8_E4M3FN, OC_BF16>(a, grid, s);
     else launch_paged_mfma<OC_FP8_E4M3FN, OC_F16>(a, grid, s);
   } else switch (p->cache_dtype) {
-    case OC_F32: hipLaunchKernelGGL(paged_portable_kernel<OC_F32>, grid, dim3(kPortThreads), 0, s, a); break;
-    case OC_F16: hipLaunchKernelGGL(paged_portable_kernel<OC_F16>, grid, dim3(kPortThreads), 0, s, a); break;
-    case OC_BF16: hipLaunchKernelGGL(paged_portable_kernel<OC_BF16>, grid, dim3(kPortThreads), 0, s, a); break;
-    default: hipLaunchKernelGGL(paged_portable_kernel<OC_FP8_E4M3FN>, grid, dim3(kPortThreads), 0, s, a);
+    case OC_F32: launch_portable<OC_F32>(a, grid, s); break;
+    case OC_F16: launch_portable<OC_F16>(a, grid, s); break;
+    case OC_BF16: launch_portable<OC_BF16>(a, grid, s); break;
+    default: launch_portable<OC_FP8_E4M3FN>(a, grid, s);
   }
   if (a.P > 1) hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)a.Hq, (unsigned)a.n), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
