@@ -27,6 +27,8 @@ inline int log2_exact(int n) {
 inline int check_mods(const oc_score_mods* m) {
   if (!std::isfinite(m->scale)) return fail(OC_ERR_INVALID, "scale %g", (double)m->scale);
   if (!(m->softcap >= 0.f) || !std::isfinite(m->softcap)) return fail(OC_ERR_INVALID, "softcap %g", (double)m->softcap);
+  if (m->softcap > 0.f && !std::isfinite(m->scale / m->softcap))
+    return fail(OC_ERR_INVALID, "scale %g over softcap %g", (double)m->scale, (double)m->softcap);
   if (m->window < 0) return fail(OC_ERR_INVALID, "window %d", m->window);
   if (m->evict && m->evict_cols < 0) return fail(OC_ERR_INVALID, "evict_cols %d", m->evict_cols);
   return OC_OK;

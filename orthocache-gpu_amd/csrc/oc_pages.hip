@@ -22,6 +22,7 @@ constexpr int kPlanWaves = kPlanThreads / kWave;
 constexpr int kMaxSeqs = 4096;   // sequences and children of a call (the plan's LDS arrays)
 constexpr int kRowThreads = 256;
 constexpr int kPagesTile = 64;
+constexpr int kMaxBlockBytes = 1 << 30;  // of a block's rows: offsets of their units stay in 32 bits
 constexpr int kMaxCols = 1 << 20, kMaxBlocks = 1 << 30;  // table columns and blocks: sums of them stay in 32 bits
 
 // Exclusive prefix sum of x over the workgroup and its total; every thread
@@ -391,6 +392,8 @@ int check_fork(const oc_fork_params* p) {
     return fail(OC_ERR_UNSUPPORTED, "over 2^30 blocks or 2^20 table columns");
   if (log2_exact(p->block_size) < 0) return fail(OC_ERR_INVALID, "block_size %d is not a power of two", p->block_size);
   if (!paged_elem_size(p->cache_dtype)) return fail(OC_ERR_INVALID, "cache dtype %d", p->cache_dtype);
+  if ((__int128)p->num_kv_heads * p->head_dim * paged_elem_size(p->cache_dtype) * p->block_size > kMaxBlockBytes)
+    return fail(OC_ERR_UNSUPPORTED, "blocks of over 2^30 bytes");
   if (!p->parents && p->num_children != p->num_seqs)
     return fail(OC_ERR_INVALID, "%d children of %d sequences need parents", p->num_children, p->num_seqs);
   return OC_OK;

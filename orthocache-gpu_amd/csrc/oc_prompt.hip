@@ -34,6 +34,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the reference that a row's sums are relative to before its first score: below every finite score
 constexpr float kNoScore = -3e38f;
 
+// What a head's scores go through: z = s (c - slope |i - j|) in base-2 units,
+// with c the raw score, or its tanh in the same units near zero (cap_scores),
+// and s = pre.  Where pre is negative or next to nothing, c is multiplied by it,
+// and s is 1.
+constexpr float kSmallest = 1e-6f;
+struct Change {
+  float s;
+  float pre;         // scale log2(e), times kTanh0 with a cap
+  float slope;       // the head's slope log2(e) / s
+  float k, inv;      // scale / cap, 1 / (kTanh0 k)
+  float lim, b1, b2; // |c| up to which the polynomial holds, its coefficients
+};
+
 struct PromptArgs {
   const char *q, *k, *v;
   char* out;
@@ -46,8 +59,8 @@ struct PromptArgs {
   const int32_t* prefix;
   const uint8_t* evict;
   int64_t e_sb, e_sh;
-  float scale, cap;
-  int32_t window;
+  Change change;  // but for the slope
+  int32_t cap, window;
   int32_t o_vec;  // out rows 8-byte aligned
   // The tiles of a workgroup's queries in shares of share_tiles (0: one share).
   // Each share's sums, of row ((b Hq + h) Sq + query) shares + share: m, l, acc.
@@ -96,19 +109,6 @@ struct Sight {
   const int* tdoc;           // LDS: documents of the tile's 64 tokens
 };
 
-// What a head's scores go through: z = s (c - slope |i - j|) in base-2 units,
-// with c the raw score, or its tanh in the same units near zero (cap_scores),
-// and s = pre.  Where pre is negative or next to nothing, c is multiplied by it,
-// and s is 1.
-constexpr float kSmallest = 1e-6f;
-struct Change {
-  float s;
-  float pre;         // scale log2(e), times kTanh0 with a cap
-  float slope;       // the head's slope log2(e) / s
-  float k, inv;      // scale / cap, 1 / (kTanh0 k)
-  float lim, b1, b2; // |c| up to which the polynomial holds, its coefficients
-};
-
 // The cap: a raw score c becomes tanh(k c) / (kTanh0 k), k = scale / cap.
 // float32 takes tanhf.  The 16-bit kernels take c (1 + b1 c^2 + b2 c^4) while
 // |k c| is at most kTanhFit (tanh(y) / y by a quadratic in y^2, fitted with a
@@ -116,6 +116,7 @@ struct Change {
 // exponential and reciprocal where a score of the wave's tile is larger: four
 // full-rate instructions against three and two quarter-rate ones.
 constexpr float kTanhFit = 0.25f;
+constexpr float kNoCap = 1e-37f;  // k below which there is no cap: 1 / k would not be finite
 constexpr float kTanh0 = 0.999999604f, kTanh1 = -0.333219082f, kTanh2 = 0.128416128f;
 
 template <int DT>
@@ -124,7 +125,7 @@ __device__ __forceinline__ void cap_scores(f32x4 (&c)[4], const Change& h) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[tb][i] = tanhf(c[tb][i] * h.k) * h.inv;
+      for (int i = 0; i < 4; ++i) c[tb][i] = h.k == 0.f ? c[tb][i] : tanhf(c[tb][i] * h.k) * h.inv;
   } else {
     float top = 0.f;
 #pragma unroll
@@ -483,23 +484,8 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
   pf_load_q<DT, D>(pa, a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh, pos0, lane, q);
   const char* kh = a.k + (int64_t)b * a.k_sb + (int64_t)kv * a.k_sh;
   const char* vh = a.v + (int64_t)b * a.v_sb + (int64_t)kv * a.v_sh;
-  Change change;
-  change.pre = a.scale * kLog2e * (CAP ? kTanh0 : 1.f);
-  change.s = change.pre < kSmallest ? 1.f : change.pre;
+  Change change = a.change;
   change.slope = BIAS ? a.slopes[h] * kLog2e / change.s : 0.f;
-  const auto same = [](float f) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f))); };
-  if constexpr (CAP) {
-    change.pre = same(change.pre);
-    change.s = same(change.s);
-  }
-  if constexpr (CAP) {
-    const float k = same(a.scale / a.cap), k2 = k * k;
-    change.k = k;
-    change.inv = same(k == 0.f ? 0.f : 1.f / (kTanh0 * k));  // (scale 0: every score is 0)
-    change.lim = same(k2 * k2 < 1e30f ? kTanhFit / fabsf(k) : -1.f);  // (k^4 has to be finite)
-    change.b1 = same(kTanh1 / kTanh0 * k2);
-    change.b2 = same(kTanh2 / kTanh0 * k2 * k2);
-  }
 
   // The tiles of the workgroup, 64 at a time, and what is true of each: that the
   // wave needs it, that all its queries see all of it (documents apart), that
@@ -737,7 +723,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs a) {
 
 template <int DT, int D>
 void launch_prompt(const PromptArgs& a, unsigned blocks, hipStream_t s) {
-  const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
+  const bool cap = a.cap != 0, bias = a.slopes != nullptr;
   auto k = cap ? (bias ? prompt_kernel<DT, D, true, true> : prompt_kernel<DT, D, true, false>)
                : (bias ? prompt_kernel<DT, D, false, true> : prompt_kernel<DT, D, false, false>);
   hipLaunchKernelGGL(k, dim3(blocks, (unsigned)a.shares), dim3(kPfThreads), 0, s, a);
@@ -765,6 +751,21 @@ int check_prompt(const oc_attend_prompt_params* p) {
     return fail(OC_ERR_INVALID, "%d query heads on %d kv heads", p->num_q_heads, p->num_kv_heads);
   if (p->kv_len > kMaxKv || p->q_len > kMaxKv) return fail(OC_ERR_UNSUPPORTED, "over 2^24 tokens");
   return check_mods(&p->mods);
+}
+
+Change change_of(float scale, float cap) {
+  Change c{};
+  c.pre = scale * kLog2e * (cap > 0.f ? kTanh0 : 1.f);
+  c.s = c.pre < kSmallest ? 1.f : c.pre;
+  if (cap > 0.f) {
+    const float ratio = scale / cap, k = std::fabs(ratio) < kNoCap ? 0.f : ratio, k2 = k * k;
+    c.k = k;
+    c.inv = 1.f / (kTanh0 * k);
+    c.lim = k2 * k2 < 1e30f ? kTanhFit / std::fabs(k) : -1.f;  // (k^4 has to be finite)
+    c.b1 = kTanh1 / kTanh0 * k2;
+    c.b2 = kTanh2 / kTanh0 * k2 * k2;
+  }
+  return c;
 }
 
 // With few queries the CUs stand idle while one workgroup after the other goes
@@ -852,7 +853,8 @@ extern "C" int oc_attend_prompt(const oc_attend_prompt_params* p, void* stream) 
   a.docs = p->kv_len ? p->documents : nullptr, a.docs_sb = p->documents_stride_b, a.ranges = (const int2*)p->workspace;
   a.slopes = p->mods.slopes, a.prefix = p->mods.prefix_lens;
   a.evict = a.T > 0 ? p->mods.evict : nullptr, a.e_sb = p->mods.evict_stride_b, a.e_sh = p->mods.evict_stride_h;
-  a.scale = p->mods.scale, a.cap = p->mods.softcap, a.window = p->mods.window;
+  a.cap = p->mods.softcap > 0.f, a.window = p->mods.window;
+  a.change = change_of(p->mods.scale, p->mods.softcap);
   const Shares shares = prompt_shares(p);
   a.shares = shares.n, a.share_tiles = shares.tiles;
   const size_t rows = ((size_t)p->batch * p->num_q_heads * p->q_len * shares.n + 3) / 4 * 4;

@@ -295,19 +295,20 @@ __global__ __launch_bounds__(kRotThreads) void append_kernel(const AppendArgs a)
   const int nt = min(a.tokens - n0, a.per);
   if (wave < nt) {
     const int row = n0 + wave;
-    int b = row, i = 0;
+    int b = row;
+    int64_t i = 0;
     bool real = true;
     if (a.cu) {
       b = seq_of_row(a.cu, a.num_seqs, row, lane);
       real = b >= 0 && row < a.cu[max(b, 0) + 1];
       b = max(b, 0);
-      i = row - a.cu[b];
+      i = (int64_t)row - a.cu[b];
     }
     const int len = a.lens[b];
     real = real && len >= 0;
     int64_t id = -2, n = 0;
     if (real) {
-      n = (int64_t)len + i;
+      n = len + i;
       const int64_t col = n >> a.block_log2;
       id = -1;
       if (col < a.max_blocks) {

@@ -7,6 +7,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -145,7 +146,15 @@ void check_caches(const Tensor& k, const Tensor& v, bool layers) {
   need(k.size(-1) <= 1 || (k.stride(-1) == 1 && v.stride(-1) == 1), "cache rows must be contiguous along head_dim");
 }
 
+// whether two tensors are known to share memory (interleaved views are not)
+bool share(const Tensor& a, const Tensor& b, bool same_counts = true) {
+  const at::MemOverlapStatus s = at::get_overlap_status(a, b);
+  return s == at::MemOverlapStatus::Partial || (same_counts && s == at::MemOverlapStatus::Full);
+}
+
 void written_caches(const Tensor& k, const Tensor& v) {
+  no_grad_needed("a written cache", k), no_grad_needed("a written cache", v);
+  need(!share(k, v), "k_cache and v_cache must be different memory");
   need(!overlaps(k) && !overlaps(v), "elements of a cache that is written may not share memory");
 }
 
@@ -227,7 +236,7 @@ py::object apply_rotary(const Tensor& q_in, const OptTensor& k_in, const Tensor&
     p.y_stride_b[i] = b < 0 ? 0 : y[i].stride(0), p.y_stride_h[i] = y[i].stride(h), p.y_stride_s[i] = y[i].stride(s);
     p.heads[i] = i32(x[i].size(1), "heads");
   }
-  need(!inplace || !k_in || x[0].data_ptr() != x[1].data_ptr() || !x[0].numel() || !x[1].numel(),
+  need(!inplace || !k_in || ((x[0].data_ptr() != x[1].data_ptr() || !x[0].numel() || !x[1].numel()) && !share(x[0], x[1])),
        "in place, q and k must be different tensors");
   p.batch = i32(batch, "batch"), p.tokens = i32(tokens, "tokens"), p.head_dim = i32(d, "head_dim");
   p.interleaved = layout == "interleaved", p.backward = backward;
@@ -366,6 +375,8 @@ Tensor attend_paged(const Tensor& q_in, const Tensor& kc, const Tensor& vc, cons
              (d <= 1 || out.stride(2) == 1) && !overlaps(out),
          "out must be a (", n, ", ", hq, ", ", d, ") ", q_in.scalar_type(), " tensor on ", on.dev.str(),
          " with a contiguous last dim and no elements that share memory");
+    no_grad_needed("attend_paged", out);
+    need(!share(out, q_in, false) && !share(out, kc) && !share(out, vc), "out may be q, but share no other memory with the inputs");
   } else {
     out = at::empty(q_in.sizes(), q_in.options().memory_format(at::MemoryFormat::Contiguous));
   }
@@ -463,6 +474,9 @@ Tables out_tables(const OutTables& out, int64_t rows, int64_t cols, int64_t bloc
       need(!(b < hi && lo < b + reach * i->element_size()), "out.", what, " overlaps an input: the old tables must stay");
     }
   };
+  const Tensor* parts[] = {&t, &l, &r, &s};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j) need(!share(*parts[i], *parts[j]), "two tensors of out share memory");
   fits(t, {rows, cols}, "block_tables"), fits(l, {rows}, "context_lens"), fits(r, {blocks}, "ref_counts"), fits(s, {1}, "status");
   return {t, l, r, s};
 }

@@ -47,12 +47,14 @@ def attend_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     (num_seqs, max_blocks); context_lens int32 (num_seqs,), the query's token
     included, clamped to 0 .. max_blocks * block_size.  evict_mask: bool or
     uint8 (num_seqs, num_kv_heads, tiles), nonzero = the complete 64-token tile
-    is left out.  num_splits: parts of each sequence (chosen by default).  The
+    is left out.  num_splits: parts of each sequence (chosen by default, 1024 at
+    most).  out: may be q, but share no other memory with the inputs.  The
     score changes are this module's.  portable: the kernel that takes every
     shape, whatever the shape.
 
     With sync, a block id outside [0, num_blocks) where a seen token needs one
-    raises ValueError; without, such tokens are left out."""
+    raises ValueError; without (as in a captured graph), such tokens are left
+    out."""
     return ops().attend_paged(q, k_cache, v_cache, block_tables, context_lens, _optional(scale), number(softcap, "softcap"),
                               alibi_slopes, window, prefix_lens, number(k_scale, "k_scale"), number(v_scale, "v_scale"),
                               evict_mask, num_splits, sync, out, portable)

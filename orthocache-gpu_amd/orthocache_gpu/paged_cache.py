@@ -17,6 +17,7 @@ from . import _native as N
 from ._ops import number, ops
 from .rotary import RotaryTable
 
+
 class OutOfPages(RuntimeError):
     """A call needs more free blocks than the cache has."""
 
@@ -42,9 +43,10 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     takes x / k_scale and x / v_scale, at most 448 in size.
 
     Sequences of one call must not share the blocks that they write
-    (`fork_pages` sees to that).  With sync, a block id outside [0, num_blocks)
-    and a table too short for a token raise ValueError; without, such tokens
-    are left out."""
+    (`fork_pages` sees to that), and k_cache and v_cache are different memory.
+    With sync, a block id outside [0, num_blocks) and a table too short for a
+    token raise ValueError; without (as in a captured graph), such tokens are
+    left out."""
     freq, scale = (None, 1.0) if table is None else (table.inv_freq, table.scale)
     return ops().append_paged(k, v, k_cache, v_cache, block_tables, context_lens, q, cu_seqlens, positions, freq, scale,
                               layout, number(k_scale, "k_scale"), number(v_scale, "v_scale"), sync)
@@ -88,9 +90,9 @@ def fork_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch
     started, and room for their next tokens.
 
     parents: int32 (num_children,), -1 for an empty sequence without blocks (a
-    later call can go on with it); a sequence that is no one's parent ends.  None: every sequence goes on.  new_tokens: how
-    many tokens each child shall have room for past its own (a number, or int32
-    (num_children,)).  Children share their parent's full blocks; a last block
+    later call can go on with it); a sequence that is no one's parent ends.
+    None: every sequence goes on.  new_tokens: how many tokens each child shall
+    have room for past its own (a number, or int32 (num_children,)).  Children share their parent's full blocks; a last block
     that is not full stays with the first child if no one else holds it, and
     the others get a copy of its tokens, in every layer: caches are
     (num_blocks, num_kv_heads, block_size, head_dim), or with layers in front.

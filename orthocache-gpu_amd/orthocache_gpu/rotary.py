@@ -16,6 +16,7 @@ import torch
 
 from ._ops import ops
 
+
 @dataclass(frozen=True)
 class RotaryTable:
     """Radians per position of every pair, float64 (rotary_dim // 2,) on the
@@ -79,7 +80,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     "interleaved" 2 i with 2 i + 1; columns from rotary_dim on are kept.
     Angles are formed in float64, the rest in float32, rounded once.
     backward: the transposed rotation, which takes the gradients of the turned
-    tensors to those of q and k.  inplace: into q and k themselves.
+    tensors to those of q and k.  inplace: into q and k themselves, which must
+    share no elements.
 
     Returns q' (and k', as a pair, when k is given)."""
     return ops().apply_rotary(q, k, positions, table.inv_freq, table.scale, layout, backward, inplace)

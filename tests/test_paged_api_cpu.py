@@ -113,6 +113,24 @@ def test_pages():
     _refused("oc_evict_pages", e, N.OC_ERR_INVALID, b"NULL")
 
 
+def test_limits():
+    from orthocache_gpu import _native as N
+    p = N.OcForkParams()
+    p.cache_dtype, p.block_size, p.num_seqs, p.num_children, p.num_kv_heads, p.head_dim = N.OC_BF16, 1 << 22, 1, 1, 2, 128
+    _refused("oc_fork_pages", p, N.OC_ERR_UNSUPPORTED, b"2^30 bytes")
+    r = N.OcAttendPromptParams()
+    r.dtype, r.batch, r.num_q_heads, r.num_kv_heads, r.q_len, r.kv_len, r.head_dim = N.OC_F16, 1, 4, 2, 8, 4096, 64
+    r.mods.scale, r.mods.softcap = 1e20, 1e-20
+    _refused("oc_attend_prompt", r, N.OC_ERR_INVALID, b"over softcap")
+    r.mods.softcap = 0.0
+    size = N.lib().oc_attend_prompt_workspace_size(ctypes.byref(r))
+    assert size % (4 * 8 * (64 + 2) * 4) == 0 and size > 0  # a whole number of shares of 4 heads of 8 queries
+    r.q = r.k = r.v = r.out = 4096
+    r.k_stride_s = r.v_stride_s = 64
+    r.workspace, r.workspace_bytes = 4104, size
+    _refused("oc_attend_prompt", r, N.OC_ERR_INVALID, b"16-byte")
+
+
 def test_entry_points_need_a_gpu():
     import orthocache_gpu as oc
     x = torch.zeros((2, 2, 64))
