@@ -5,6 +5,8 @@
 // queries, updates the online softmax, and adds V^T P^T.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "oc_kernels.h"
 #include "orthocache_hip.h"
 
@@ -362,7 +364,7 @@ __device__ __forceinline__ void pf_logits(const PfQ<DT, D>& q, const char* sk, i
 // causal rows past the output tolerance.
 // float32: 16x16x4 steps over (tb, i), A = V[16tb + 4r + i][16nc + x], B =
 // c[tb][i], exact.
-// PK: float16 pairs by one instruction (the same rounding).
+// PK: pairs by one instruction (the same rounding).
 template <int DT, int D, bool HILO = DT == OC_BF16, bool PK = false>
 __device__ __forceinline__ void pf_pv(f32x4 (&acc)[D / 16], const f32x4 (&c)[4], const char* svb, int lane) {
   const int x = lane & 15;
@@ -392,18 +394,19 @@ __device__ __forceinline__ void pf_pv(f32x4 (&acc)[D / 16], const f32x4 (&c)[4],
       uint32_t bhi[4], blo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (DT == OC_BF16) {
+        if constexpr (PK) {
+          static_assert(!HILO, "pairs are rounded once");
+          typedef float f32x2 __attribute__((ext_vector_type(2)));
+          typedef std::conditional_t<DT == OC_BF16, __bf16, _Float16> T;
+          typedef T pair __attribute__((ext_vector_type(2)));
+          bhi[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{pv[2 * e], pv[2 * e + 1]}), pair));
+        } else if constexpr (DT == OC_BF16) {
           const __bf16 h0 = (__bf16)pv[2 * e], h1 = (__bf16)pv[2 * e + 1];
           bhi[e] = (uint32_t)__builtin_bit_cast(uint16_t, h0) | ((uint32_t)__builtin_bit_cast(uint16_t, h1) << 16);
           if constexpr (HILO) {
             const __bf16 l0 = (__bf16)(pv[2 * e] - (float)h0), l1 = (__bf16)(pv[2 * e + 1] - (float)h1);
             blo[e] = (uint32_t)__builtin_bit_cast(uint16_t, l0) | ((uint32_t)__builtin_bit_cast(uint16_t, l1) << 16);
           }
-        } else if constexpr (PK) {
-          static_assert(!HILO, "pairs are rounded once");
-          typedef float f32x2 __attribute__((ext_vector_type(2)));
-          typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-          bhi[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{pv[2 * e], pv[2 * e + 1]}), f16x2));
         } else {
           const _Float16 h0 = (_Float16)pv[2 * e], h1 = (_Float16)pv[2 * e + 1];
           bhi[e] = (uint32_t)__builtin_bit_cast(uint16_t, h0) | ((uint32_t)__builtin_bit_cast(uint16_t, h1) << 16);

@@ -221,8 +221,10 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
   }
   float s = h.s;
   mt = __builtin_fmaf(mt, s, -off);
-  mt = fmaxf(mt, xpair<16>(mt));
-  mt = fmaxf(mt, xpair<32>(mt));
+  float lo, hi;  // over the query's four lanes: a lane's own and its partner's, in either order
+  row_pair<16>(mt, lo, hi);
+  row_pair<32>(fmaxf(lo, hi), lo, hi);
+  mt = fmaxf(lo, hi);
   // Far from zero the maximum's rounding is no longer small against 1, and the
   // fma below would see it: there the scores are rounded like the maximum.
   if (__builtin_amdgcn_ballot_w64(fabsf(mt) > 16777216.f)) {
@@ -363,9 +365,16 @@ struct PromptFetch {
   int k, v;
 
   __device__ static __forceinline__ PromptFetch of(const PrefillArgs& a, int tid) {
-    const int r = tid / L::LPT, c = tid % L::LPT;
-    return {r * (int)a.k_ss + 16 * (c ^ L::swz(r)),
+    const int r = (unsigned)tid / L::LPT, c = tid & (L::LPT - 1), swz = (unsigned)r / L::RB % L::LPT;
+    return {r * (int)a.k_ss + 16 * (c ^ swz),
             DT == OC_F32 ? r * (int)a.v_ss + 16 * c : pf_vtok(r) * (int)a.v_ss + 16 * (c ^ (2 * L::vswz(r)))};
+  }
+
+  // n within 0 .. most, in scalar registers (the compiler's clamp is a vector instruction, and so then are the products)
+  __device__ static __forceinline__ int rows_of(int n, int most) {
+    n = min(n, most);
+    asm("" : "+s"(n));
+    return max(n, 0);
   }
 
   // tile t straight to LDS, rows at or past kv_len as zeros; by the first wave
@@ -376,7 +385,7 @@ struct PromptFetch {
     const int wbase = __builtin_amdgcn_readfirstlane(tid & ~63);
 #pragma unroll
     for (int j = 0; j < L::NL; ++j) {
-      const int row = 64 * t + STEP * j, n = max(min(a.Skv - row, 64 - STEP * j), 0);
+      const int row = 64 * t + STEP * j, n = rows_of(a.Skv - row, 64 - STEP * j);
       const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
           (void*)pf_uniform(kh + (int64_t)row * (int)a.k_ss), (short)0, __builtin_amdgcn_readfirstlane(n * (int)a.k_ss), 0x00020000);
       const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
