@@ -132,7 +132,7 @@ __device__ __forceinline__ void cap_scores(f32x4 (&c)[4], const Change& h) {
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(c[tb][i]));
-    if (__builtin_amdgcn_ballot_w64(top > h.lim)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > h.lim) != 0, 0)) {
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
@@ -158,7 +158,7 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
                                                const Sight& e, int tok0, bool full) {
   float mt = -__builtin_inff();
   if constexpr (CAP) cap_scores<DT>(c, h);
-  if (h.pre < kSmallest) {
+  if (__builtin_expect(h.pre < kSmallest, 0)) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb) c[tb] *= h.pre;
   }
@@ -187,7 +187,7 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
         for (int i = 0; i < 4; ++i) c[tb][i] = __builtin_fmaf(-h.slope, fabsf(d0 - (float)(16 * tb + i)), c[tb][i]);
     }
   }
-  if (full) {
+  if (__builtin_expect(full, 1)) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
@@ -227,7 +227,7 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
   mt = fmaxf(lo, hi);
   // Far from zero the maximum's rounding is no longer small against 1, and the
   // fma below would see it: there the scores are rounded like the maximum.
-  if (__builtin_amdgcn_ballot_w64(fabsf(mt) > 16777216.f)) {
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(fabsf(mt) > 16777216.f) != 0, 0)) {
 #pragma unroll
     for (int tb = 0; tb < 4; ++tb)
 #pragma unroll
@@ -236,7 +236,7 @@ __device__ __forceinline__ void prompt_softmax(PfState& st, f32x4 (&acc)[D / 16]
     off = 0.f;
   }
   const bool move = mt > st.m + kPfSlack;
-  if (__builtin_amdgcn_ballot_w64(move)) {
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(move) != 0, 0)) {
     const float mn = move ? mt : st.m;
     const float alpha = __builtin_amdgcn_exp2f(st.m - mn);
     st.m = mn;
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
             first(pa, kh, vh, docs, n.t, tid, nk, nv, nd);
           }
         }
-        if (cur.need) {
+        if (__builtin_expect(cur.need, 1)) {
           f32x4 c[4];
           pf_logits<DT, D>(q, ck, lane, c);
           const Sight eye{w_lo, window, prefix, docs && !cur.one ? sqdoc + 16 * wave : nullptr, cd};
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(DT =
         if (!ANY && cur.border && bad_tile[0] == cur.t) return true;
         const Tile n = next_tile();
         if (n.t < t_hi) fetch(n.t);  // in flight during this tile
-        if (cur.need) {
+        if (__builtin_expect(cur.need, 1)) {
           f32x4 c[4];
           pf_logits<DT, D>(q, stage_k(0), lane, c);
           const Sight eye{w_lo, window, prefix, docs && !cur.one ? sqdoc + 16 * wave : nullptr, sdoc0};

@@ -10,6 +10,9 @@
 // of the first and of the second half of a row, or 16 bytes of interleaved
 // pairs.  Bound by the bytes (one read, one write) but for few tokens, where
 // the chain of dependent loads (sequence, length, block id) is what is left.
+// Measured: 4096 tokens of 32 + 8 heads of 128 in bf16 14.9 us (84 MB, 5.6
+// TB/s); the same heads into pages, 16 tokens 5.5 us, 4762 into fp8 33.5 us
+// (137 MB, 4.1 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -421,6 +424,7 @@ void launch_append(bool vec, bool inter, unsigned blocks, hipStream_t s, const A
 }
 
 // tokens per workgroup: kRotTokens once every CU has two workgroups of them
+// (1, 2, 4 tokens: 40, 36, 33.5 us for 4762 into pages; 5.7, 6.2, 9.3 for 16)
 int tokens_per_group(int64_t tokens) { return tokens >= (int64_t)2 * kRotTokens * device_cus() ? kRotTokens : 1; }
 
 }  // namespace
