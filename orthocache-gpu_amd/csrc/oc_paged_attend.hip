@@ -111,6 +111,9 @@ constexpr int kPortHeads = 4;  // query heads of a workgroup
 // lane i has the scores of token i.  p.V: the tokens seen are put together in
 // LDS, and a lane adds up four columns (twice four above head_dim 256) of every
 // TP-th of them, TP as many rows as 64 lanes hold, VA rows of loads ahead.
+// Bound by latency more than bytes: float32, 16 x 4096 tokens, 32 / 8 heads, 84
+// us (4.3 TB/s); float32 queries on an fp8 cache, 5 x 94499 tokens, 48 us (2.2
+// TB/s; 208 with a lane per token and one V row at a time).
 template <int CT, int NI>
 __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const PagedArgs a) {
   constexpr int ES = Elem<CT>::size;
@@ -345,7 +348,10 @@ __global__ __launch_bounds__(kPortThreads) void paged_portable_kernel(const Page
 //   operand, is the lane's own eight probabilities.
 //
 // Bound by the bytes of K and V: a unit of 32 tokens of 128 columns is 16 KiB
-// of loads to about 500 cycles of work.
+// of loads to about 500 cycles of work.  Measured with the join: 16 sequences of
+// up to 32768 tokens, 32 / 8 heads, bf16, 1.41 GB in 241 us (5.9 TB/s; the
+// portable kernel 290); 4 of up to 131072, 64 / 8 heads, fp8, 0.84 GB in 153 us
+// (5.5 TB/s; portable 379).
 
 constexpr int kPmWaves = 4;
 constexpr int kPmThreads = kPmWaves * kWave;
@@ -753,14 +759,23 @@ bool paged_tuned(const oc_attend_paged_params* p) {
   return true;
 }
 
-// Shares of a sequence: about four workgroups per CU, at least four tiles each.
+// Shares of a sequence: four workgroups per CU, of eight tiles or more (four
+// while there is not one for every CU); eight per CU where that leaves 32 tiles
+// each.  Measured on 256 CUs (bf16, head_dim
+// 128, 8 kv heads; shares: us): 16 x 32768 tokens 8: 253, 16: 241, 32: 246; 128 x
+// 4096 1: 246, 2: 239, 4: 242; 16 x 4096 4: 44, 8: 46, 16: 49; 4 x 8192 8: 31,
+// 16: 26, 32: 30; 1 x 32768 32: 32, 64: 30, 128: 34; fp8, 4 x 131072 16: 165, 32:
+// 154, 64: 154, 128: 171; 3 x 300 1: 9.4, 2: 11.4; f16, one kv head, 2 x 17782
+// 34: 17.3, 69: 14.5.
 int paged_splits(const oc_attend_paged_params* p) {
   const int64_t tiles = ((int64_t)p->max_blocks * p->block_size + 63) / 64;
   if (p->num_splits > 0) return (int)std::max<int64_t>(1, std::min<int64_t>({p->num_splits, tiles, kMaxSplits}));
   const int64_t g = p->num_q_heads / p->num_kv_heads;
   const int heads = paged_tuned(p) ? kPmHeads : kPortHeads;
   const int64_t blocks = (int64_t)p->num_seqs * p->num_kv_heads * ((g + heads - 1) / heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({4 * (int64_t)device_cus() / std::max<int64_t>(blocks, 1), tiles / 4, kMaxSplits}));
+  const int64_t cus = device_cus(), b = std::max<int64_t>(blocks, 1), four = 4 * cus / b, eight = 8 * cus / b;
+  const int64_t n = eight > 0 && tiles / eight >= 32 ? eight : std::min(four, std::max(tiles / 8, std::min(tiles / 4, cus / b)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
 }
 
 template <int CT>
