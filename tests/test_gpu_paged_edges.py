@@ -153,3 +153,25 @@ def test_two_calls_at_once():
         torch.cuda.synchronize()
         for g, w in zip(got, want):
             assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.02, 0.3, 7.0, 1e-25, 1e25, 1e38])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+def test_append_fp8_quotients(dt, scale):
+    """What an fp8 page holds is the rounded quotient, byte for byte: signed zeros, ties, the clamp, infinities, NaN."""
+    import orthocache_gpu as oc
+    g = torch.Generator().manual_seed(3)
+    n, d = 64, 128
+    x = torch.randn((n, 1, d), generator=g) * torch.exp2(torch.randint(-14, 12, (n, 1, d), generator=g).float()) * scale
+    ties = torch.arange(-256, 256).float() / 16 * scale
+    x.view(-1)[:512] = ties
+    x.view(-1)[512:524] = torch.tensor([0.0, -0.0, float("inf"), -float("inf"), float("nan"), 448 * scale, -448 * scale, 449 * scale,
+                                        464 * scale, 3e38, -3e38, 1e-38])
+    x = x.to(dt).to(DEV)
+    kc, vc = (torch.zeros((4, 1, 16, d), dtype=torch.float8_e4m3fn, device=DEV) for _ in range(2))
+    oc.append_paged(x, x, kc, vc, _i32([[0, 1, 2, 3]]), _i32([0]), cu_seqlens=_i32([0, n]), k_scale=scale, v_scale=scale)
+    want = (x.float() / torch.tensor(scale, dtype=torch.float32, device=DEV)).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    for c in (kc, vc):
+        got = c.view(torch.uint8).view(n, 1, d)
+        same = (got == want) | (((got & 127) == 127) & ((want & 127) == 127))  # (a NaN of either sign)
+        assert bool(same.all()), (x[~same][:4], got[~same][:4], want[~same][:4])
