@@ -806,7 +806,7 @@ Shares prompt_shares(const oc_attend_prompt_params* p) {
   // the most tiles that a workgroup sees, and those of one in the middle
   const int64_t most = p->mods.window > 0 && !p->mods.prefix_lens
                            ? std::min<int64_t>(all, ((int64_t)p->mods.window + kPfRows + 63) / 64 + 1) : all;
-  const int64_t mean = std::min<int64_t>(most, std::max<int64_t>(1, (p->kv_len - p->q_len / 2 + 64) / 64));
+  const int64_t mean = std::min<int64_t>(most, (p->kv_len - std::min(p->q_len, p->kv_len) / 2 + 64) / 64);
   const int64_t cus = device_cus(), room = f32 && wide ? cus : 2 * cus;
   const int64_t tiles = std::max<int64_t>(f32 ? 4 : 8, (blocks * mean + room - 1) / room);
   if (blocks >= 2 * cus || 2 * most < 3 * tiles) return {0, 1};

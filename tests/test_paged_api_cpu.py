@@ -125,6 +125,10 @@ def test_limits():
     r.mods.softcap = 0.0
     size = N.lib().oc_attend_prompt_workspace_size(ctypes.byref(r))
     assert size % (4 * 8 * (64 + 2) * 4) == 0 and size > 0  # a whole number of shares of 4 heads of 8 queries
+    r.num_q_heads = r.num_kv_heads = 1
+    for r.q_len, r.kv_len in ((65408, 32768), (64, 1 << 24), (30000, 40000), (2 ** 23, 64)):  # shares' sums stay small
+        assert N.lib().oc_attend_prompt_workspace_size(ctypes.byref(r)) < 2 ** 27
+    r.num_q_heads, r.num_kv_heads, r.q_len, r.kv_len = 4, 2, 8, 4096
     r.q = r.k = r.v = r.out = 4096
     r.k_stride_s = r.v_stride_s = 64
     r.workspace, r.workspace_bytes = 4104, size
